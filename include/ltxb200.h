@@ -199,6 +199,61 @@ int ltx_attention_ws(const void* q, int64_t ldq, const void* k, int64_t ldk, con
                      const void* gate_logits, int64_t ld_gate, void* workspace, size_t workspace_bytes, int dtype,
                      void* stream);
 
+/* Attention with a per-sample key mask (sdpa's mask argument, ltx_nn.py:22-26, for masks
+ * that do not depend on the query: a padded text context): operands as ltx_attention.
+ * mask: (B, Tk) with ld_mask elements between samples (0: one mask for all samples);
+ * LTX_MASK_BOOL bytes, 0 = the key is left out; LTX_MASK_F32 / LTX_MASK_BF16 values added to
+ * the scaled scores, a key being left out at or below half of the type's lowest finite
+ * value (-inf included). K and V of a left-out key do not reach the output, whatever they
+ * hold. A row without keys (or whose scores are all -inf) is zero. scale > 0. bf16: head_dim
+ * 64 or 128; fp32: 32, 64 or 128. */
+typedef enum { LTX_MASK_BOOL = 0, LTX_MASK_F32 = 1, LTX_MASK_BF16 = 2 } ltx_mask_kind;
+int ltx_attention_masked(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
+                         int64_t ldo, int B, int64_t Tq, int64_t Tk, int heads, int head_dim, float scale,
+                         const void* mask, int64_t ld_mask, int mask_kind, const void* gate_logits, int64_t ld_gate,
+                         int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------- */
+/* Rows in 8-bit floating point, and linear layers on them. No counterpart in the       */
+/* reference, which runs its nn.Linear layers in bf16 (ltx_nn.py:126-158, 188-192,       */
+/* 244-245).                                                                            */
+/* An "8-bit row" matrix (rows, cols) is e4m3 data, row-major with a row stride ldq that  */
+/* is a multiple of 16 bytes, and one power-of-two scale per row and block of 128       */
+/* columns: value = e4m3(data[r][c]) * 2^(code - 127), code = byte (c / 128) % 4 of the    */
+/* 32-bit word                                                                          */
+/*   scales[(c / 512) * P + (r / 128) * 128 + (r % 32) * 4 + (r % 128) / 32],            */
+/* P = rows rounded up to 256. data and scales are 16-byte aligned; scales hold          */
+/* ltx_fp8_scale_bytes(rows, cols) bytes (0 for sizes that are not positive).             */
+/* ---------------------------------------------------------------------------------- */
+size_t ltx_fp8_scale_bytes(int64_t rows, int64_t cols);
+/* x (rows, cols) F32 or BF16 -> 8-bit rows. The scale of a block is the least power of
+ * two s >= 2^-126 with max|x| <= 448 s over its finite values (1 for a block of zeros), the
+ * data x / s rounded to the nearest e4m3; NaN and infinities become the 8-bit NaN. Bytes
+ * of a row from cols up to the next multiple of 16 are written as zeros. Any ldx >= cols
+ * (16-byte loads when x is 16-byte aligned and ldx a multiple of 8). */
+int ltx_quantize_fp8(const void* x, int64_t ldx, int64_t rows, int64_t cols, void* q, int64_t ldq, void* scales,
+                     int dtype, void* stream);
+/* 8-bit rows -> x (rows, cols) F32 or BF16; exact in both as long as the value is a normal
+ * number of the type. */
+int ltx_dequantize_fp8(const void* q, int64_t ldq, const void* scales, int64_t rows, int64_t cols, void* x,
+                       int64_t ldx, int dtype, void* stream);
+/* Scales given as fp32 powers of two, s (rows, ceil(cols / 128)) with row stride ld, into
+ * the word layout above (the exponent field is taken; other values are the caller's
+ * error). For weights stored in 8 bits by other programs. */
+int ltx_fp8_pack_scales(const float* s, int64_t ld, int64_t rows, int64_t cols, void* scales, void* stream);
+/* ltx_norm_modulate with the result as 8-bit rows: norm(x) * (1 + scale) + shift in fp32
+ * (table + mod unrounded), rounded once, to 8 bits. D a multiple of 8, at most 16384. */
+int ltx_norm_modulate_fp8(const void* x, int64_t ldx, void* q, int64_t ldq, void* scales, int64_t rows,
+                          int64_t rows_per_batch, int D, int norm_kind, float eps, const ltx_modulation* mod,
+                          int dtype, void* stream);
+/* C = epilogue(A W^T + bias), A (M, K) and W (N, K) 8-bit rows, C (M, N) and the epilogue's
+ * vectors in `dtype`; the epilogue kinds of ltx_linear, in fp32 and rounded once (residual +
+ * gate * (acc + bias) with the gate's table + mod unrounded). Any ldc >= N; silu_input is
+ * rejected. C may be the epilogue's residual. */
+int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, const void* W, int64_t ldw, const void* w_scales,
+                   void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, const ltx_epilogue* epi, int dtype,
+                   void* stream);
+
 /* ---------------------------------------------------------------------------------- */
 /* Denoise update: X0 conversion + CFG guidance + Euler step.                          */
 /* Replaces guided_denoise_step's X0 (ltx_dit.py:591-593), guide (ltx_dit.py:551-562,  */

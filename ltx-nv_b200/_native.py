@@ -215,6 +215,17 @@ _SIGNATURES = {
                                              c_vp]),
     "ltx_attention_merge": (ctypes.c_int, [c_vp, c_vp, ctypes.c_int, c_i64, ctypes.c_int, ctypes.c_int, c_vp, c_i64,
                                            c_vp, c_i64, c_vp]),
+    "ltx_attention_masked": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, ctypes.c_int, c_i64,
+                                            c_i64, ctypes.c_int, ctypes.c_int, ctypes.c_float, c_vp, c_i64,
+                                            ctypes.c_int, c_vp, c_i64, ctypes.c_int, c_vp]),
+    "ltx_fp8_scale_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
+    "ltx_quantize_fp8": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, ctypes.c_int, c_vp]),
+    "ltx_dequantize_fp8": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, ctypes.c_int, c_vp]),
+    "ltx_fp8_pack_scales": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
+    "ltx_norm_modulate_fp8": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, ctypes.c_int, ctypes.c_int,
+                                             ctypes.c_float, ctypes.POINTER(Modulation), ctypes.c_int, c_vp]),
+    "ltx_linear_fp8": (ctypes.c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                      ctypes.POINTER(Epilogue), ctypes.c_int, c_vp]),
     "ltx_ctx_create": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(c_vp)]),
     "ltx_ctx_destroy": (ctypes.c_int, [c_vp]),
     "ltx_dit_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DitConfig), c_i64, c_i64]),
@@ -544,6 +555,151 @@ def attention_merge(o_parts: torch.Tensor, lse_parts: torch.Tensor, gate_logits:
         raise ValueError("o_parts (R, rows, H*d) and lse_parts (R, rows, H) must be contiguous")
     _call("ltx_attention_merge", _ptr(o_parts), _ptr(lse_parts), r, rows, heads, head_dim, _ptr(gate_logits),
           _ld(gate_logits) if gate_logits is not None else 0, _ptr(out), _ld(out), _stream(out))
+
+
+# ---------------------------------------------------------------------------------------
+# 8-bit rows (fp8) and masked attention
+# ---------------------------------------------------------------------------------------
+
+
+def _on(t: torch.Tensor, name: str, *args, label: str | None = None) -> None:
+    """_call with the stream of t's device appended, made on that device (which need not be
+    the current one)."""
+    dev = t.device
+    if dev.index == torch.cuda.current_device():
+        _call(name, *args, torch.cuda.current_stream(dev).cuda_stream, label=label)
+        return
+    with torch.cuda.device(dev):
+        _call(name, *args, torch.cuda.current_stream(dev).cuda_stream, label=label)
+
+
+def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
+    if not first.is_cuda:
+        raise ValueError("libltxb200 kernels take CUDA tensors only")
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+
+
+class Fp8Rows:
+    """A (rows, cols) matrix in 8-bit floating point with a power-of-two scale per row and
+    block of 128 columns (the 8-bit rows of include/ltxb200.h). `data` is a (rows, cols)
+    float8_e4m3fn view whose row stride is a multiple of 16, `scales` the packed scale
+    words; both are owned by this object and reused by every call that is given it."""
+
+    __slots__ = ("data", "scales", "rows", "cols")
+
+    def __init__(self, rows: int, cols: int, device: torch.device | str):
+        ld = (cols + 15) // 16 * 16
+        data = torch.empty(rows, ld, dtype=torch.float8_e4m3fn, device=device)
+        self.data = data if ld == cols else data[:, :cols]
+        self.scales = torch.empty((rows + 255) // 256 * 256 * ((cols + 511) // 512), dtype=torch.int32, device=device)
+        self.rows, self.cols = rows, cols
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @classmethod
+    def from_parts(cls, data: torch.Tensor, scales: torch.Tensor) -> "Fp8Rows":
+        """8-bit rows from e4m3 values (rows, cols) and float32 power-of-two scales (rows,
+        ceil(cols / 128)), as a checkpoint of 8-bit weights holds them. The values are
+        copied; scales that are not powers of two in [2^-126, 2^127] are rejected (one
+        device-to-host check: for weights at load time, not for a captured graph)."""
+        if data.dim() != 2 or data.dtype != torch.float8_e4m3fn:
+            raise ValueError("data must be a (rows, cols) float8_e4m3fn tensor")
+        rows, cols = data.shape
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (rows, (cols + 127) // 128):
+            raise ValueError(f"scales must be float32 ({rows}, {(cols + 127) // 128}), one per 128 columns")
+        if rows == 0 or cols == 0:
+            raise ValueError("a matrix of 8-bit rows has at least one row and one column")
+        bits = scales.contiguous().view(torch.int32)
+        if bool(((bits & 0x807FFFFF) != 0).any() | (bits == 0).any() | (bits == 0x7F800000).any()):
+            raise ValueError("scales must be powers of two in [2^-126, 2^127]")
+        _same_device(data, scales)
+        out = cls(rows, cols, data.device)
+        out.data.copy_(data)
+        s = scales.contiguous()
+        _on(data, "ltx_fp8_pack_scales", s.data_ptr(), s.shape[1], rows, cols, out.scales.data_ptr())
+        return out
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The (rows, cols) values in `dtype` (float32 or bfloat16; exact in both)."""
+        out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.data.device)
+        dt = _dt(out)
+        if out.numel():
+            _on(out, "ltx_dequantize_fp8", self.data.data_ptr(), self.data.stride(0), self.scales.data_ptr(), self.rows,
+                self.cols, out.data_ptr(), self.cols, dt)
+        return out
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+    """x (rows, cols) float32 or bfloat16, unit column stride -> 8-bit rows."""
+    dt, ld = _dt(x), _ld(x)
+    _same_device(x)
+    out = Fp8Rows(x.shape[0], x.shape[1], x.device)
+    if x.numel():
+        _on(x, "ltx_quantize_fp8", x.data_ptr(), ld, x.shape[0], x.shape[1], out.data.data_ptr(), out.data.stride(0),
+            out.scales.data_ptr(), dt)
+    return out
+
+
+def norm_modulate_fp8(x: torch.Tensor, rows_per_batch: int, kind: int, eps: float, mod: Modulation | None) -> Fp8Rows:
+    """norm_modulate with the result as 8-bit rows."""
+    dt, ld = _dt(x), _ld(x)
+    _same_device(x)
+    rows, d = x.shape
+    out = Fp8Rows(rows, d, x.device)
+    if x.numel():
+        _on(x, "ltx_norm_modulate_fp8", x.data_ptr(), ld, out.data.data_ptr(), out.data.stride(0),
+            out.scales.data_ptr(), rows, rows_per_batch, d, kind, eps, ctypes.byref(mod) if mod is not None else None, dt)
+    return out
+
+
+def linear_fp8(a: Fp8Rows, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = None) -> None:
+    """c = epilogue(a @ w.T (+ bias)); a (M, K) and w (N, K) 8-bit rows, c (M, N) a row-major
+    view in the epilogue's type."""
+    if a.cols != w.cols or tuple(c.shape) != (a.rows, w.rows):
+        raise ValueError(f"shape mismatch a{a.shape} w{w.shape} c{tuple(c.shape)}")
+    dt, ld = _dt(c), _ld(c)
+    _same_device(c, a.data, w.data)
+    if c.numel():
+        _on(c, "ltx_linear_fp8", a.data.data_ptr(), a.data.stride(0), a.scales.data_ptr(), w.data.data_ptr(),
+            w.data.stride(0), w.scales.data_ptr(), c.data_ptr(), ld, a.rows, w.rows, a.cols,
+            ctypes.byref(epi) if epi is not None else None, dt,
+            label=f"linear_fp8 M={a.rows} N={w.rows} K={a.cols}" if _profile is not None else None)
+
+
+MASK_KINDS = {torch.bool: 0, torch.float32: 1, torch.bfloat16: 2}
+
+
+def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, batch: int, tq: int, tk: int,
+                     heads: int, head_dim: int, scale: float, mask: torch.Tensor,
+                     gate_logits: torch.Tensor | None = None) -> None:
+    """attention with a key mask (batch, tk), or (1, tk) for all samples: bool (True: the key
+    takes part) or an additive float32 / bfloat16 one."""
+    if mask.dtype not in MASK_KINDS:
+        raise TypeError(f"unsupported mask dtype {mask.dtype}; bool, float32 or bfloat16")
+    if mask.dim() != 2 or mask.shape[1] != tk or mask.shape[0] not in (1, batch) or (tk > 1 and mask.stride(1) != 1):
+        raise ValueError(f"mask must be a row-major ({batch} or 1, {tk}) view, got {tuple(mask.shape)}")
+    dt = _dt(q)
+    for name, t, rows in (("k", k, batch * tk), ("v", v, batch * tk), ("o", o, batch * tq), ("q", q, batch * tq)):
+        if t.dtype != q.dtype:
+            raise TypeError(f"{name} is {t.dtype}, q is {q.dtype}")
+        if t.shape[0] != rows or t.shape[1] < heads * head_dim:
+            raise ValueError(f"{name} must have {rows} rows of at least {heads * head_dim} columns")
+    if gate_logits is not None and (gate_logits.dtype != q.dtype or gate_logits.shape[0] != batch * tq
+                                    or gate_logits.shape[1] < heads):
+        raise ValueError(f"gate_logits must be {q.dtype} ({batch * tq}, >= {heads})")
+    _same_device(q, k, v, o, mask, gate_logits)
+    _on(q, "ltx_attention_masked", q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), o.data_ptr(), _ld(o),
+        batch, tq, tk, heads, head_dim, scale, mask.data_ptr(), 0 if mask.shape[0] == 1 else mask.stride(0),
+        MASK_KINDS[mask.dtype], _ptr(gate_logits), _ld(gate_logits) if gate_logits is not None else 0, dt,
+        label=f"attention_masked B={batch} H={heads} Tq={tq} Tk={tk} d={head_dim}" if _profile is not None else None)
 
 
 def cfg_euler(vel: torch.Tensor, latent: torch.Tensor, timesteps: torch.Tensor, cfg_scale: float, sigma: float,

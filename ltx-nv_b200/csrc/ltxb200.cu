@@ -4,7 +4,9 @@
 #include "philox.cu"
 #include "elementwise.cu"
 #include "gemm.cu"
+#include "fp8.cu"
 #include "attention.cu"
+#include "cross_attention.cu"
 #include "parallel.cu"
 #include "vae.cu"
 #include "dit_step.cu"

@@ -24,6 +24,7 @@ import numpy
 import torch
 
 import _native as nat
+from _native import Fp8Rows
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -41,17 +42,218 @@ def rms_norm(x: torch.Tensor, eps: float = 1e-6, weight: torch.Tensor | None = N
 
 
 def sdpa(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor | None = None) -> torch.Tensor:
-    """ltx_nn.py:22-26: q, k, v (B, H, T, d) -> (B, H, T, d), non-causal, no mask."""
-    if mask is not None:
-        raise NotImplementedError("attention masks are not used by the LTX DiT path")
+    """ltx_nn.py:22-26: q, k, v (B, H, T, d) -> (B, H, T, d), non-causal. mask: one that does
+    not depend on the query or the head, (B or 1, 1, 1, Tk), (B or 1, Tk) or (Tk,), bool
+    (True: the key takes part) or additive; see cross_attention."""
     b, h, tq, d = q.shape
     tk = k.shape[2]
-    qt = q.transpose(1, 2).reshape(b * tq, h * d).contiguous()
-    kt = k.transpose(1, 2).reshape(b * tk, h * d).contiguous()
-    vt = v.transpose(1, 2).reshape(b * tk, h * d).contiguous()
+
+    def rows(x, t):
+        return x.transpose(1, 2).reshape(b, t, h * d)
+
+    if mask is not None:
+        o = cross_attention(rows(q, tq), rows(k, tk), rows(v, tk), h, mask=mask)
+        return o.view(b, tq, h, d).transpose(1, 2)
+    qt, kt, vt = (rows(x, t).reshape(b * t, h * d).contiguous() for x, t in ((q, tq), (k, tk), (v, tk)))
     o = torch.empty_like(qt)
     nat.attention(qt, kt, vt, o, b, tq, tk, h, d, d ** -0.5, None)
     return o.view(b, tq, h, d).transpose(1, 2)
+
+
+# ---------------------------------------------------------------------------------------
+# Attention to another sequence under a key mask
+# ---------------------------------------------------------------------------------------
+
+
+def key_mask(mask: torch.Tensor, batch: int, tk: int) -> torch.Tensor:
+    """A mask over the keys as the (B or 1, Tk) row-major view that nat.attention_masked
+    takes, from (Tk,), (B or 1, Tk) or (B or 1, 1, 1, Tk)."""
+    if mask.dim() == 4:
+        if mask.shape[1] != 1 or mask.shape[2] != 1:
+            raise NotImplementedError(f"masks that depend on the query or the head, got {tuple(mask.shape)}")
+        mask = mask[:, 0, 0]
+    elif mask.dim() == 1:
+        mask = mask[None]
+    if mask.dim() != 2 or mask.shape[1] != tk or mask.shape[0] not in (1, batch):
+        raise ValueError(f"a key mask is ({batch} or 1, 1, 1, {tk}), ({batch} or 1, {tk}) or ({tk},), got "
+                         f"{tuple(mask.shape)}")
+    return mask if tk == 1 or mask.stride(1) == 1 else mask.contiguous()
+
+
+def _row_major(x: torch.Tensor) -> torch.Tensor:
+    """x (B, T, W) as a (B * T, W) row-major view; a copy only where there is no such view."""
+    if x.dim() != 3:
+        raise ValueError(f"expected (batch, tokens, width), got {tuple(x.shape)}")
+    x2 = x.reshape(-1, x.shape[-1])
+    return x2 if x2.stride(1) == 1 else x2.contiguous()
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int,
+                    mask: torch.Tensor | None = None, gate_logits: torch.Tensor | None = None,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T * scale + mask) v per sample and head: q (B, Tq, H*d), k and v (B, Tk,
+    H*d) token-major (column views of packed projections are taken as they are), out (B, Tq,
+    H*d), optionally times 2 * sigmoid(gate_logits), gate_logits (B, Tq, H) (ltx_nn.py:22-26,
+    231-235).
+
+    mask (key_mask's shapes): bool, True where a key takes part; or float32 / bfloat16, added
+    to the scores, a key being left out where it is at or below half of the type's lowest
+    finite value. What k and v hold at a key that is left out does not matter. A sample
+    without any key gives zeros (torch's softmax would give NaN, or a mean over the padding
+    for masks of the lowest value). Without a mask this is the framework's attention."""
+    b, tq, width = q.shape
+    tk = k.shape[1]
+    if heads <= 0 or width % heads:
+        raise ValueError(f"the width {width} is not a multiple of {heads} heads")
+    if tuple(k.shape) != (b, tk, width) or tuple(v.shape) != (b, tk, width):
+        raise ValueError(f"k and v must be ({b}, Tk, {width}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if gate_logits is not None and tuple(gate_logits.shape) != (b, tq, heads):
+        raise ValueError(f"gate_logits must be ({b}, {tq}, {heads}), got {tuple(gate_logits.shape)}")
+    if out is None:
+        out = torch.empty(b, tq, width, device=q.device, dtype=q.dtype)
+    elif tuple(out.shape) != (b, tq, width) or not out.is_contiguous() or out.dtype != q.dtype:
+        raise ValueError(f"out must be a contiguous {q.dtype} ({b}, {tq}, {width}) tensor")
+    if mask is not None:
+        mask = key_mask(mask, b, tk)
+    if out.numel() == 0:
+        return out
+    if tk == 0:
+        return out.zero_()
+    d = width // heads
+    g = _row_major(gate_logits) if gate_logits is not None else None
+    args = (_row_major(q), _row_major(k), _row_major(v), out.view(b * tq, width), b, tq, tk, heads, d,
+            d ** -0.5 if scale is None else float(scale))
+    if mask is None:
+        nat.attention(*args, g)
+    else:
+        nat.attention_masked(*args, mask, g)
+    return out
+
+
+# ---------------------------------------------------------------------------------------
+# 8-bit rows: linear layers and the norm in front of them
+# ---------------------------------------------------------------------------------------
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+    """x (..., K) float32 or bfloat16 -> its (rows, K) matrix of 8-bit rows: e4m3 values with
+    a power-of-two scale per 128 columns. Weights (N, K) are quantised with it once."""
+    x2 = x.reshape(-1, x.shape[-1])
+    return nat.quantize_fp8(x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous())
+
+
+def _modulation(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None):
+    """nat.Modulation of shift / scale vectors given per sample (B, D) or per token (B, T, D),
+    and the tensors that it points to. One descriptor addresses both vectors from the lower
+    of their addresses, with one stride; vectors that do not share it are copied."""
+    b, t, d = x.shape
+    held = {}
+    for name, vec in (("shift", shift), ("scale", scale)):
+        if vec is None:
+            continue
+        if tuple(vec.shape) not in ((b, d), (b, t, d)) or any(v.dim() != vec.dim() for v in held.values()):
+            raise ValueError(f"{name} must be ({b}, {d}) or ({b}, {t}, {d}), like the other vector, got "
+                             f"{tuple(vec.shape)}")
+        if vec.dtype != x.dtype or vec.device != x.device:
+            raise ValueError(f"{name} must be {x.dtype} on {x.device}")
+        held[name] = vec
+    if not held:
+        return None, held
+    vecs = list(held.values())
+    st = vecs[0].stride()
+    if any(v.stride() != st or v.stride(-1) != 1 or v.data_ptr() % 32 for v in vecs) or any(i % 8 for i in st[:-1]):
+        held = {name: torch.empty(vec.shape, dtype=vec.dtype, device=vec.device).copy_(vec)
+                for name, vec in held.items()}
+        st = next(iter(held.values())).stride()
+    base = min(v.data_ptr() for v in held.values())
+    m = nat.Modulation()
+    m.mod = base
+    m.mod_ld_batch, m.mod_ld_tok = st[0], (st[1] if len(st) == 3 else 0)
+    for name, vec in held.items():
+        setattr(m, "has_" + name, 1)
+        setattr(m, name + "_mod_off", (vec.data_ptr() - base) // vec.element_size())
+    return m, held
+
+
+_NORM_KINDS = {"rms": nat.LTX_NORM_RMS, "layer": nat.LTX_NORM_LAYER, "none": nat.LTX_NORM_NONE}
+
+
+def norm_modulate_fp8(x: torch.Tensor, scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
+                      kind: str = "rms", eps: float = 1e-6) -> Fp8Rows:
+    """norm(x) * (1 + scale) + shift of x (B, T, D) as (B * T, D) 8-bit rows, the operand of
+    linear_fp8: fp32 arithmetic and one rounding. scale and shift (B, D) or (B, T, D) in x's
+    type; kind "rms", "layer" or "none"; D a multiple of 8."""
+    if kind not in _NORM_KINDS:
+        raise ValueError(f"kind must be one of {sorted(_NORM_KINDS)}, got {kind!r}")
+    x2 = _row_major(x)
+    mod, held = _modulation(x, shift, scale)
+    out = nat.norm_modulate_fp8(x2, max(x.shape[1], 1), _NORM_KINDS[kind], eps, mod)
+    del held  # the vectors live until the launch; the allocator keeps stream order after it
+    return out
+
+
+_ACTIVATIONS = {None: nat.EPI_NONE, "gelu_tanh": nat.EPI_GELU_TANH, "silu": nat.EPI_SILU}
+
+
+def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activation: str | None = None,
+               residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+               dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """activation(x W^T + bias), or residual + gate * (x W^T + bias), with both operands in
+    8-bit rows and fp32 sums, rounded once to `dtype`.
+
+    x: (..., K) float32 or bfloat16, quantised here (quantize_fp8), or its Fp8Rows already
+    (from norm_modulate_fp8). weight: (N, K) Fp8Rows. The result is (..., N), or (rows, N) /
+    residual's shape for an Fp8Rows x, in `dtype` (default: x's type, residual's, or
+    bfloat16). gate: (B, N) per sample or (B, T, N) per token of a (B, T, N) residual; bias,
+    residual and gate are in `dtype`. out may be the residual itself."""
+    if not isinstance(weight, Fp8Rows):
+        raise TypeError("weight must be Fp8Rows (quantize_fp8 or Fp8Rows.from_parts)")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")
+    if gate is not None and residual is None:
+        raise ValueError("a gate needs a residual")
+    if activation is not None and residual is not None:
+        raise ValueError("an activation and a residual exclude each other")
+    n = weight.rows
+    if isinstance(x, Fp8Rows):
+        lead = tuple(residual.shape[:-1]) if residual is not None else \
+            tuple(out.shape[:-1]) if out is not None else (x.rows,)
+        dtype = dtype or (residual.dtype if residual is not None else out.dtype if out is not None else torch.bfloat16)
+        cols = x.cols
+    else:
+        lead, dtype, cols = tuple(x.shape[:-1]), dtype or x.dtype, x.shape[-1]
+    if cols != weight.cols:
+        raise ValueError(f"x has {cols} columns, the weight {weight.cols}")
+    shape = (*lead, n)
+    if isinstance(x, Fp8Rows) and math.prod(lead) != x.rows:
+        raise ValueError(f"{x.rows} rows do not fill {shape}")
+    for name, t, want in (("bias", bias, (n,)), ("residual", residual, shape), ("out", out, shape)):
+        if t is not None and (tuple(t.shape) != want or t.dtype != dtype or t.device != x.device):
+            raise ValueError(f"{name} must be {dtype} {want} on {x.device}, got {t.dtype} {tuple(t.shape)}")
+    kind, rpb, mod = _ACTIVATIONS[activation], 1, None
+    if residual is not None:
+        kind = nat.EPI_GATE_RESIDUAL
+        residual2 = residual.reshape(-1, n)
+        residual2 = residual2 if residual2.stride(1) == 1 else residual2.contiguous()
+        if gate is not None:
+            if residual.dim() != 3 or tuple(gate.shape) not in ((lead[0], n), shape):
+                raise ValueError(f"gate must be (B, N) or (B, T, N) of a (B, T, N) residual, got {tuple(gate.shape)}")
+            if gate.dtype != dtype or gate.device != x.device:
+                raise ValueError(f"gate must be {dtype} on {x.device}")
+            gate = gate.contiguous()
+            rpb = max(lead[1], 1)
+            per_tok = gate.dim() == 3
+            mod = nat.modulation(None, gate, shift=None, scale=(0, 0), mod_ld_batch=rpb * n if per_tok else n,
+                                 mod_ld_tok=n if per_tok else 0)
+    if out is None:
+        out = torch.empty(shape, device=x.device, dtype=dtype)
+    elif not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    rows = x if isinstance(x, Fp8Rows) else quantize_fp8(x)
+    nat.linear_fp8(rows, weight, out.view(-1, n),
+                   nat.epilogue(kind, bias=bias.contiguous() if bias is not None else None,
+                                residual=residual2 if residual is not None else None, gate=mod, rows_per_batch=rpb))
+    return out
 
 
 # ---------------------------------------------------------------------------------------

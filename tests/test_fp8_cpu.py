@@ -1,0 +1,169 @@
+"""Refusals of the 8-bit row and masked-attention entry points, and their host arithmetic:
+no GPU is touched (every check comes before the first CUDA call)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import _native as nat
+import fp8_reference as ref
+import ltx_nn
+
+INVALID, UNSUPPORTED = 1, 3
+P = 4096  # a 16-byte aligned address that no call gets to use
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return nat.load_library()
+
+
+def test_reference_rounding_matches_torch():
+    x = torch.randn(64, 300).to(torch.bfloat16)
+    want, s = ref.quantize(x)
+    s = s.repeat_interleave(128, 1)[:, :300]
+    assert torch.equal((x.float() / s.float()).to(torch.float8_e4m3fn).double() * s, want)
+
+
+def test_scale_bytes(lib):
+    assert lib.ltx_fp8_scale_bytes(1, 1) == 256 * 4
+    assert lib.ltx_fp8_scale_bytes(256, 512) == 256 * 4
+    assert lib.ltx_fp8_scale_bytes(257, 513) == 512 * 2 * 4
+    assert lib.ltx_fp8_scale_bytes(0, 5) == 0 and lib.ltx_fp8_scale_bytes(5, -1) == 0
+    r = nat.Fp8Rows(257, 513, "cpu")
+    assert r.scales.numel() * 4 == lib.ltx_fp8_scale_bytes(257, 513)
+    assert r.data.shape == (257, 513) and r.data.stride(0) == 528
+
+
+@pytest.mark.parametrize("change,msg", [
+    ({"x": None}, b"x must be"), ({"q": None}, b"non-NULL"), ({"scales": None}, b"non-NULL"),
+    ({"rows": 0}, b"positive"), ({"cols": 0}, b"positive"), ({"rows": 1 << 31}, b"out of range"),
+    ({"ldq": 511}, b"multiple of 16"), ({"ldq": 496}, b"multiple of 16"), ({"ldx": 511}, b"ldx"),
+    ({"q": P + 8}, b"16-byte"), ({"scales": P + 4}, b"16-byte"), ({"x": P + 1}, b"aligned"), ({"dtype": 2}, b"dtype")])
+def test_quantize_refusals(lib, change, msg):
+    a = {"x": P, "ldx": 512, "rows": 4, "cols": 512, "q": P, "ldq": 512, "scales": P, "dtype": 1, "stream": None} | change
+    assert lib.ltx_quantize_fp8(*a.values()) == INVALID
+    assert msg in lib.ltx_last_error()
+    a = {"q": a["q"], "ldq": a["ldq"], "scales": a["scales"], "rows": a["rows"], "cols": a["cols"], "x": a["x"],
+         "ldx": a["ldx"], "dtype": a["dtype"], "stream": None}
+    assert lib.ltx_dequantize_fp8(*a.values()) == INVALID
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"x": None}, INVALID), ({"D": 100}, INVALID), ({"D": 16392, "ldx": 16392, "ldq": 16400}, UNSUPPORTED),
+    ({"ldx": 500}, INVALID), ({"x": P + 2}, INVALID), ({"rpb": 0}, INVALID), ({"kind": 3}, INVALID),
+    ({"q": P + 1}, INVALID), ({"rows": 0}, INVALID), ({"dtype": 5}, INVALID)])
+def test_norm_refusals(lib, change, status):
+    a = {"x": P, "ldx": 512, "q": P, "ldq": 512, "scales": P, "rows": 4, "rpb": 2, "D": 512, "kind": 0, "eps": 1e-6,
+         "mod": None, "dtype": 1, "stream": None} | change
+    assert lib.ltx_norm_modulate_fp8(*a.values()) == status, lib.ltx_last_error()
+
+
+@pytest.mark.parametrize("change,msg", [
+    ({"A": None}, b"A:"), ({"Ws": None}, b"W:"), ({"C": None}, b"C must"), ({"M": 0}, b"positive"),
+    ({"lda": 250}, b"multiple of 16"), ({"ldw": 240}, b"hold the columns"), ({"ldc": 63}, b"ldc"), ({"C": P + 1}, b"aligned"),
+    ({"dtype": 7}, b"dtype"), ({"N": 1 << 31, "ldc": 1 << 31}, b"out of range")])
+def test_linear_refusals(lib, change, msg):
+    a = {"A": P, "lda": 256, "As": P, "W": P, "ldw": 256, "Ws": P, "C": P, "ldc": 64, "M": 4, "N": 64, "K": 256,
+         "epi": None, "dtype": 1, "stream": None} | change
+    assert lib.ltx_linear_fp8(*a.values()) == INVALID
+    assert msg in lib.ltx_last_error(), lib.ltx_last_error()
+
+
+@pytest.mark.parametrize("fields,msg", [
+    ({"kind": 9}, b"kind"), ({"silu_input": 1}, b"silu_input"), ({"kind": nat.EPI_GATE_RESIDUAL}, b"residual"),
+    ({"kind": nat.EPI_GATE_RESIDUAL, "residual": P, "ld_residual": 63}, b"ld_residual"),
+    ({"kind": nat.EPI_ROW_MASK_ADD}, b"row_mask"), ({"bias": P + 1}, b"aligned")])
+def test_linear_epilogue_refusals(lib, fields, msg):
+    e = nat.Epilogue()
+    for k, v in fields.items():
+        setattr(e, k, v)
+    st = lib.ltx_linear_fp8(P, 256, P, P, 256, P, P, 64, 4, 64, 256, ctypes.byref(e), 1, None)
+    assert st == INVALID and msg in lib.ltx_last_error(), lib.ltx_last_error()
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"mask": None}, INVALID), ({"q": None}, INVALID), ({"B": 0}, INVALID), ({"Tk": 0}, INVALID),
+    ({"heads": 0}, INVALID), ({"d": 96, "ldq": 400}, UNSUPPORTED), ({"d": 32}, UNSUPPORTED), ({"ldk": 120}, INVALID),
+    ({"ldo": 132}, INVALID), ({"v": P + 8}, INVALID), ({"ld_mask": 99}, INVALID), ({"kind": 3}, INVALID),
+    ({"kind": 1, "mask": P + 2}, INVALID), ({"scale": 0.0}, INVALID), ({"scale": float("inf")}, INVALID),
+    ({"scale": float("nan")}, INVALID), ({"gate": P, "ld_gate": 1}, INVALID), ({"B": 1 << 20}, INVALID),
+    ({"Tq": 1 << 31}, INVALID), ({"dtype": 2}, INVALID)])
+def test_masked_attention_refusals(lib, change, status):
+    a = {"q": P, "ldq": 128, "k": P, "ldk": 128, "v": P, "ldv": 128, "o": P, "ldo": 128, "B": 2, "Tq": 5, "Tk": 100,
+         "heads": 2, "d": 64, "scale": 0.125, "mask": P, "ld_mask": 100, "kind": 0, "gate": None, "ld_gate": 0,
+         "dtype": 1, "stream": None} | change
+    assert lib.ltx_attention_masked(*a.values()) == status, lib.ltx_last_error()
+
+
+def test_python_entry_points_refuse_bad_arguments():
+    x = torch.zeros(2, 3, 256, dtype=torch.bfloat16)
+    w = nat.Fp8Rows(64, 256, "cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        ltx_nn.quantize_fp8(x)
+    with pytest.raises(TypeError):
+        ltx_nn.quantize_fp8(x.half())
+    with pytest.raises(ValueError, match="columns"):
+        ltx_nn.linear_fp8(x[..., :128], w)
+    with pytest.raises(TypeError, match="Fp8Rows"):
+        ltx_nn.linear_fp8(x, x)
+    with pytest.raises(ValueError, match="activation"):
+        ltx_nn.linear_fp8(x, w, activation="relu")
+    res = torch.zeros(2, 3, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="exclude"):
+        ltx_nn.linear_fp8(x, w, activation="silu", residual=res)
+    with pytest.raises(ValueError, match="gate needs"):
+        ltx_nn.linear_fp8(x, w, gate=res)
+    with pytest.raises(ValueError, match="residual must"):
+        ltx_nn.linear_fp8(x, w, residual=res.float())
+    with pytest.raises(ValueError, match="gate must"):
+        ltx_nn.linear_fp8(x, w, residual=res, gate=torch.zeros(3, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="bias must"):
+        ltx_nn.linear_fp8(x, w, bias=torch.zeros(63, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="contiguous"):
+        ltx_nn.linear_fp8(x, w, out=torch.zeros(2, 64, 3, dtype=torch.bfloat16).transpose(1, 2))
+    with pytest.raises(ValueError, match="do not fill"):
+        ltx_nn.linear_fp8(nat.Fp8Rows(7, 256, "cpu"), w, residual=res)
+    with pytest.raises(ValueError, match="kind"):
+        ltx_nn.norm_modulate_fp8(x, kind="batch")
+    with pytest.raises(ValueError, match="scale must"):
+        ltx_nn.norm_modulate_fp8(x, scale=torch.zeros(2, 255, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="like the other"):
+        ltx_nn.norm_modulate_fp8(x, scale=torch.zeros(2, 256, dtype=torch.bfloat16), shift=x)
+    with pytest.raises(ValueError, match="float8"):
+        nat.Fp8Rows.from_parts(x[0], torch.ones(3, 2))
+    with pytest.raises(ValueError, match="one per 128"):
+        nat.Fp8Rows.from_parts(torch.zeros(3, 256).to(torch.float8_e4m3fn), torch.ones(3, 3))
+
+
+def test_masks_refused():
+    q, k = torch.zeros(2, 5, 128, dtype=torch.bfloat16), torch.zeros(2, 9, 128, dtype=torch.bfloat16)
+    ones = torch.ones(2, 9, dtype=torch.bool)
+
+    def call(mask, **kw):
+        return ltx_nn.cross_attention(q, k, k, 2, mask=mask, **kw)
+
+    with pytest.raises(NotImplementedError, match="depend on the query"):
+        call(torch.ones(2, 1, 5, 9, dtype=torch.bool))
+    with pytest.raises(NotImplementedError):
+        ltx_nn.sdpa(*(x.view(2, -1, 2, 64).transpose(1, 2) for x in (q, k, k)), mask=torch.ones(2, 2, 1, 9))
+    for bad in (ones[:, :8], torch.ones(3, 9, dtype=torch.bool), torch.ones(2, 1, 9, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="key mask"):
+            call(bad)
+    with pytest.raises(TypeError, match="mask dtype"):
+        call(ones.to(torch.int32))
+    with pytest.raises(TypeError, match="mask dtype"):
+        call(ones.half())
+    with pytest.raises(ValueError, match="CUDA"):
+        call(ones)
+    with pytest.raises(ValueError, match="gate_logits"):
+        call(ones, gate_logits=q[..., :3])
+    with pytest.raises(ValueError, match="heads"):
+        ltx_nn.cross_attention(q, k, k, 3, mask=ones)
+    with pytest.raises(ValueError, match="k and v"):
+        ltx_nn.cross_attention(q, k, k[:, :8], 2, mask=ones)
+    with pytest.raises(TypeError):
+        ltx_nn.cross_attention(q, k.float(), k, 2, mask=ones)
+    with pytest.raises(ValueError, match="out must"):
+        call(ones, out=torch.zeros(2, 5, 128))
