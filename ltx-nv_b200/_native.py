@@ -10,6 +10,7 @@ rejected, the error propagates.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from pathlib import Path
 
@@ -582,23 +583,22 @@ def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
 
 
 class Fp8Rows:
-    """A (rows, cols) matrix in 8-bit floating point with a power-of-two scale per row and
-    block of 128 columns (the 8-bit rows of include/ltxb200.h). `data` is a (rows, cols)
-    float8_e4m3fn view whose row stride is a multiple of 16, `scales` the packed scale
-    words; both are owned by this object and reused by every call that is given it."""
+    """A (..., cols) tensor in 8-bit floating point with a power-of-two scale per row and
+    block of 128 columns (the 8-bit rows of include/ltxb200.h). `shape` is the tensor's,
+    `data` its (rows, cols) float8_e4m3fn view whose row stride is a multiple of 16, `scales`
+    the packed scale words; both are owned by this object and reused by every call that is
+    given it."""
 
-    __slots__ = ("data", "scales", "rows", "cols")
+    __slots__ = ("data", "scales", "rows", "cols", "shape")
 
-    def __init__(self, rows: int, cols: int, device: torch.device | str):
+    def __init__(self, *shape: int, device: torch.device | str):
+        *lead, cols = shape
+        rows = math.prod(lead)
         ld = (cols + 15) // 16 * 16
         data = torch.empty(rows, ld, dtype=torch.float8_e4m3fn, device=device)
         self.data = data if ld == cols else data[:, :cols]
         self.scales = torch.empty((rows + 255) // 256 * 256 * ((cols + 511) // 512), dtype=torch.int32, device=device)
-        self.rows, self.cols = rows, cols
-
-    @property
-    def shape(self) -> tuple[int, int]:
-        return self.rows, self.cols
+        self.rows, self.cols, self.shape = rows, cols, tuple(shape)
 
     @property
     def device(self) -> torch.device:
@@ -621,15 +621,15 @@ class Fp8Rows:
         if bool(((bits & 0x807FFFFF) != 0).any() | (bits == 0).any() | (bits == 0x7F800000).any()):
             raise ValueError("scales must be powers of two in [2^-126, 2^127]")
         _same_device(data, scales)
-        out = cls(rows, cols, data.device)
+        out = cls(rows, cols, device=data.device)
         out.data.copy_(data)
         s = scales.contiguous()
         _on(data, "ltx_fp8_pack_scales", s.data_ptr(), s.shape[1], rows, cols, out.scales.data_ptr())
         return out
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The (rows, cols) values in `dtype` (float32 or bfloat16; exact in both)."""
-        out = torch.empty(self.rows, self.cols, dtype=dtype, device=self.data.device)
+        """The values in `dtype` (float32 or bfloat16; exact in both)."""
+        out = torch.empty(self.shape, dtype=dtype, device=self.data.device)
         dt = _dt(out)
         if out.numel():
             _on(out, "ltx_dequantize_fp8", self.data.data_ptr(), self.data.stride(0), self.scales.data_ptr(), self.rows,
@@ -637,23 +637,24 @@ class Fp8Rows:
         return out
 
 
-def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
-    """x (rows, cols) float32 or bfloat16, unit column stride -> 8-bit rows."""
+def quantize_fp8(x: torch.Tensor, shape: tuple[int, ...] | None = None) -> Fp8Rows:
+    """x (rows, cols) float32 or bfloat16, unit column stride -> 8-bit rows (of `shape`)."""
     dt, ld = _dt(x), _ld(x)
     _same_device(x)
-    out = Fp8Rows(x.shape[0], x.shape[1], x.device)
+    out = Fp8Rows(*(shape or x.shape), device=x.device)
     if x.numel():
         _on(x, "ltx_quantize_fp8", x.data_ptr(), ld, x.shape[0], x.shape[1], out.data.data_ptr(), out.data.stride(0),
             out.scales.data_ptr(), dt)
     return out
 
 
-def norm_modulate_fp8(x: torch.Tensor, rows_per_batch: int, kind: int, eps: float, mod: Modulation | None) -> Fp8Rows:
-    """norm_modulate with the result as 8-bit rows."""
+def norm_modulate_fp8(x: torch.Tensor, rows_per_batch: int, kind: int, eps: float, mod: Modulation | None,
+                      shape: tuple[int, ...] | None = None) -> Fp8Rows:
+    """norm_modulate with the result as 8-bit rows (of `shape`)."""
     dt, ld = _dt(x), _ld(x)
     _same_device(x)
     rows, d = x.shape
-    out = Fp8Rows(rows, d, x.device)
+    out = Fp8Rows(*(shape or x.shape), device=x.device)
     if x.numel():
         _on(x, "ltx_norm_modulate_fp8", x.data_ptr(), ld, out.data.data_ptr(), out.data.stride(0),
             out.scales.data_ptr(), rows, rows_per_batch, d, kind, eps, ctypes.byref(mod) if mod is not None else None, dt)

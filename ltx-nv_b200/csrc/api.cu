@@ -101,6 +101,35 @@ static CUtensorMap encode_tmap_bf16_2d(const void* ptr, uint64_t inner, uint64_t
   return m;
 }
 
+static CUtensorMap encode_tmap_2d(CUtensorMapDataType type, const void* ptr, uint64_t inner, uint64_t outer,
+                                  uint64_t ld_bytes, uint32_t box_inner, uint32_t box_outer,
+                                  CUtensorMapSwizzle swizzle) {
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || ld_bytes % 16 != 0)
+    throw ApiError{LTX_ERR_INVALID, "TMA operand and row stride must be multiples of 16 bytes"};
+  auto fn = encode_fn();
+  if (fn == nullptr) throw ApiError{LTX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable"};
+  CUtensorMap m;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {ld_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(&m, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    throw ApiError{LTX_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit rows) failed with code " + std::to_string(int(r))};
+  return m;
+}
+
+CUtensorMap make_tmap_u8_2d(const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_outer) {
+  return encode_tmap_2d(CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, inner, outer, ld, 128, box_outer,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+CUtensorMap make_tmap_u32_2d(const void* ptr, uint64_t inner, uint64_t outer, uint32_t box_inner) {
+  return encode_tmap_2d(CU_TENSOR_MAP_DATA_TYPE_UINT32, ptr, inner, outer, inner * 4, box_inner, 1,
+                        CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 CUtensorMap make_tmap_bf16_4d(const void* ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
                               const uint32_t (&box)[4]) {
   if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)

@@ -179,79 +179,265 @@ LTX_DEVICE float gelu_sigmoid(float v) {
   return __fdividef(v, 1.f + __expf(-z2));
 }
 
-// Epilogue of one accumulator in fp32, rounded once on the store:
-// v + bias, then the activation, residual + gate * v, or v + row_vec on marked rows.
+// Epilogue of eight accumulators (columns [col, col + 8) of row `row`, sample sb, token st)
+// in fp32, rounded once on the store: acc + bias, then the activation, residual + gate *
+// (acc + bias), or + row_vec on marked rows. `vec`: 16-byte accesses are allowed.
 template <typename T>
-LTX_DEVICE float fp8_epilogue1(const Epi<T>& e, int64_t row, int64_t col, float v) {
-  if (e.bias) v += ld_elem<T>(e.bias + col);
-  switch (e.kind) {
-    case LTX_EPI_GELU_TANH:
-      return gelu_sigmoid(v);
-    case LTX_EPI_SILU:
-      return __fdividef(v, 1.f + __expf(-v));
-    case LTX_EPI_GATE_RESIDUAL: {
-      float g = 1.f;
-      if (e.gate.on) {
-        const int64_t b = row / e.rows_per_batch, t = row - b * e.rows_per_batch;
-        g = 0.f;
-        if (e.gate.table) g += ld_elem<T>(e.gate.table + e.gate.toff + col);
-        if (e.gate.mod) g += ld_elem<T>(e.gate.mod + b * e.gate.ldb + t * e.gate.ldt + e.gate.moff + col);
-      }
-      return fmaf(g, v, ld_elem<T>(e.residual + row * e.ld_res + col));
+LTX_DEVICE void fp8_epilogue8(const Epi<T>& e, bool vec, T* __restrict__ crow, int64_t row, int64_t sb, int64_t st,
+                              int col, int N, float (&v)[8]) {
+  const bool whole = vec && col + 8 <= N;
+  auto load = [&](const T* p, float (&x)[8]) {
+    if (whole) {
+      ld8<T>(p, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = col + i < N ? ld_elem<T>(p + i) : 0.f;
     }
-    case LTX_EPI_ROW_MASK_ADD:
-      return e.row_mask[row] > 0.f ? v + ld_elem<T>(e.row_vec + col) : v;
-    default:
-      return v;
+  };
+  float a[8];
+  if (e.bias) {
+    load(e.bias + col, a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += a[i];
+  }
+  if (e.kind == LTX_EPI_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu_sigmoid(v[i]);
+  } else if (e.kind == LTX_EPI_SILU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fdividef(v[i], 1.f + __expf(-v[i]));
+  } else if (e.kind == LTX_EPI_GATE_RESIDUAL) {
+    float g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = e.gate.on ? 0.f : 1.f;
+    if (e.gate.table) {
+      load(e.gate.table + e.gate.toff + col, a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] += a[i];
+    }
+    if (e.gate.mod) {
+      load(e.gate.mod + sb * e.gate.ldb + st * e.gate.ldt + e.gate.moff + col, a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] += a[i];
+    }
+    load(e.residual + row * e.ld_res + col, a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(g[i], v[i], a[i]);
+  } else if (e.kind == LTX_EPI_ROW_MASK_ADD && e.row_mask[row] > 0.f) {
+    load(e.row_vec + col, a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += a[i];
+  }
+  if (whole) {
+    st8<T>(crow + col, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < N) st_elem<T>(crow + col + i, v[i]);
   }
 }
 
-// Plain form of the product: 64x64 tile, 32 columns of K at a time, values scaled as they
-// are staged in shared memory, fp32 sums.
+// ---------------------------------------------------------------------------------
+// C = epilogue(A W^T) on 8-bit rows with the block-scaled tensor-core MMA.
+//
+// acc[m][n] = sum over blocks b of 2^(ea[m][b] + ew[n][b]) sum_{k in b} a[m][k] w[n][k]: the MMA
+// takes e4m3 operands and a power of two per row and 32 values of K, so a block of 128
+// columns is one 128-byte slab of both operands and four MMAs (K = 32) that read the same
+// scale byte; sums stay in fp32 in tensor memory, no scaling is left for the CUDA cores.
+// A scale word holds four blocks, so scales move once per four slabs: 512 bytes per 128
+// rows by TMA next to the slab, then one tcgen05.cp into tensor memory, ordered with the
+// MMAs that follow it; two scale buffers alternate.
+// ---------------------------------------------------------------------------------
+
+// One 128 x 128 tile per CTA, K split over the CTAs of a cluster (SPLIT = cluster size),
+// whose fp32 partial tiles are added through distributed shared memory in rank order:
+// short and wide problems spread over the SMs without a workspace or a second launch,
+// and the sum's order does not depend on timing.
+struct Fp8TileCfg {
+  static constexpr int STAGES = 6;
+  static constexpr int SLAB = 128 * 128;             // 128 rows x 128 bytes
+  static constexpr int SF = 512;                     // scale words of 128 rows, one quad
+  static constexpr int STAGE_BYTES = 2 * SLAB + 2 * SF;
+  static constexpr int TMEM_COLS = 256;              // accumulator [0, 128), scales [128, 144)
+  static constexpr int LD_PART = 128 + 4;            // floats per row of a partial tile (no bank conflicts)
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
+  static_assert(128 * LD_PART * 4 <= STAGES * STAGE_BYTES, "the partial tile reuses the operand ring");
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-    linear_fp8_simt_kernel(const uint8_t* __restrict__ A, int64_t lda, const uint32_t* __restrict__ As,
-                           int64_t a_padded, const uint8_t* __restrict__ W, int64_t ldw,
-                           const uint32_t* __restrict__ Ws, int64_t w_padded, T* __restrict__ C, int64_t ldc, int M,
-                           int N, int K, Epi<T> epi) {
-  __shared__ float sa[32][64 + 4];
-  __shared__ float sw[32][64 + 4];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int64_t m0 = int64_t(blockIdx.y) * 64, n0 = int64_t(blockIdx.x) * 64;
-  float acc[4][4] = {};
-  auto value = [&](const uint8_t* p, int64_t ld, const uint32_t* s, int64_t padded, int64_t r, int k) {
-    float lo, hi;
-    fp8_unpack2(p[r * ld + k], lo, hi);
-    const uint32_t word = s[fp8_word(r, k / kFp8Quad, padded)];
-    return lo * fp8_scale((word >> (8 * ((k / kFp8Block) & 3))) & 255);
-  };
-  for (int k0 = 0; k0 < K; k0 += 32) {
-    for (int e = tid; e < 64 * 32; e += 256) {
-      const int r = e >> 5, kk = e & 31;
-      const bool in = k0 + kk < K;
-      sa[kk][r] = in && m0 + r < M ? value(A, lda, As, a_padded, m0 + r, k0 + kk) : 0.f;
-      sw[kk][r] = in && n0 + r < N ? value(W, ldw, Ws, w_padded, n0 + r, k0 + kk) : 0.f;
+__global__ void __launch_bounds__(192, 1)
+    gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                         T* __restrict__ C, int64_t ldc, int M, int N, int K, int split, int vec, Epi<T> epi) {
+  using Cfg = Fp8TileCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES);
+  uint64_t* empty = full + Cfg::STAGES;
+  uint64_t* tfull = empty + Cfg::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = warp_id(), lane = lane_id();
+  // the CTAs of a cluster are neighbours in x: rank = blockIdx.x % split
+  const int tile = int(blockIdx.x) / split, rank = int(blockIdx.x) - tile * split;
+  const int n_tiles = (N + 127) / 128;
+  const int m0 = (tile / n_tiles) * 128, n0 = (tile % n_tiles) * 128;
+  const int k_blocks = (K + 127) / 128;
+  const int kb0 = int(int64_t(k_blocks) * rank / split), kb1 = int(int64_t(k_blocks) * (rank + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 32; ++kk) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[kk][ty * 4 + i], sw[kk][tx * 4 + j], acc[i][j]);
-    }
-    __syncthreads();
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmSB);
   }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int it = kb - kb0, s = it % Cfg::STAGES;
+        if (!mbar_wait(&empty[s], (uint32_t(it / Cfg::STAGES) & 1) ^ 1, abort_flag)) break;
+        uint8_t* st = smem + s * Cfg::STAGE_BYTES;
+        const bool sf = kb == kb0 || (kb & 3) == 0;  // a new scale word
+        mbar_arrive_expect_tx(&full[s], sf ? Cfg::STAGE_BYTES : 2 * Cfg::SLAB);
+        tma_load_2d(st, &tmA, &full[s], kb * 128, m0);
+        tma_load_2d(st + Cfg::SLAB, &tmB, &full[s], kb * 128, n0);
+        if (sf) {
+          tma_load_2d(st + 2 * Cfg::SLAB, &tmSA, &full[s], m0, kb >> 2);
+          tma_load_2d(st + 2 * Cfg::SLAB + Cfg::SF, &tmSB, &full[s], n0, kb >> 2);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int it = kb - kb0, s = it % Cfg::STAGES;
+        if (!mbar_wait(&full[s], uint32_t(it / Cfg::STAGES) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + s * Cfg::STAGE_BYTES), b = a + Cfg::SLAB;
+        const uint32_t sfa = tmem + 128u + uint32_t((kb >> 2) & 1) * 8u, sfb = sfa + 4u;
+        if (kb == kb0 || (kb & 3) == 0) {
+          tmem_cp_scales(sfa, umma_desc_rows16(a + 2 * Cfg::SLAB));
+          tmem_cp_scales(sfb, umma_desc_rows16(a + 2 * Cfg::SLAB + Cfg::SF));
+        }
+        const uint32_t idesc = umma_idesc_mx8(128, 128, kb & 3);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= M) continue;
+        for (int k = 0; k < 4; ++k)
+          umma_mx8_ss(tmem, umma_desc_sw128(a + k * 32, 16, 1024), umma_desc_sw128(b + k * 32, 16, 1024), idesc, sfa,
+                      sfb, (it > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&empty[s]);
+      }
+      if (ok) umma_commit(tfull);
+    }
+  } else {
+    const int q = warp & 3;  // TMEM lane quadrant
+    const int64_t m = int64_t(m0) + q * 32 + lane;
+    const bool live = m < M;
+    ok = mbar_wait(tfull, 0, abort_flag);
+    if (ok) {
+      tc_fence_after();
+      const uint32_t tbase = tmem + (uint32_t(q * 32) << 16);
+      float* part = reinterpret_cast<float*>(smem) + (q * 32 + lane) * Cfg::LD_PART;
+      const int64_t sb = m / epi.rows_per_batch, st = m - sb * epi.rows_per_batch;
+#pragma unroll 1
+      for (int c0 = 0; c0 < 128 && n0 + c0 < N; c0 += 32) {
+        uint32_t rr[32];
+        tmem_ld32(tbase + uint32_t(c0), rr);
+        tmem_wait_ld();
+        if (!live) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (n < N) st_elem<T>(C + m * ldc + n, fp8_epilogue1<T>(epi, m, n, acc[i][j]));
+        for (int j = 0; j < 4; ++j) {
+          if (split > 1) {
+            // every MMA of this CTA has read its operands: the ring is free
+            *reinterpret_cast<uint4*>(part + c0 + 8 * j) = make_uint4(rr[8 * j], rr[8 * j + 1], rr[8 * j + 2], rr[8 * j + 3]);
+            *reinterpret_cast<uint4*>(part + c0 + 8 * j + 4) =
+                make_uint4(rr[8 * j + 4], rr[8 * j + 5], rr[8 * j + 6], rr[8 * j + 7]);
+          } else if (n0 + c0 + 8 * j < N) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(rr[8 * j + e]);
+            fp8_epilogue8<T>(epi, vec, C + m * ldc, m, sb, st, n0 + c0 + 8 * j, N, v);
+          }
+        }
+      }
     }
   }
+  __syncwarp();
+  if (split > 1) {
+    cluster_sync_all();
+    // CTA `rank` finishes the tile's column groups of 8 with index % split == rank
+    const int rows = min(128, M - m0), groups = (min(128, N - n0) + 7) / 8;
+    const int mine = (groups - rank + split - 1) / split;
+    const uint32_t base = smem_u32(smem);
+    for (int i = threadIdx.x; i < rows * mine; i += blockDim.x) {
+      const int r = i / mine, c = ((i - r * mine) * split + rank) * 8;
+      float v[8] = {};
+      for (int p = 0; p < split; ++p) {
+        const uint32_t at = mapa_shared(base, uint32_t(p)) + uint32_t(r * Cfg::LD_PART + c) * 4u;
+        const float4 x = ld_cluster_f4(at), y = ld_cluster_f4(at + 16);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+      const int64_t m = int64_t(m0) + r;
+      const int64_t sb = m / epi.rows_per_batch, st = m - sb * epi.rows_per_batch;
+      fp8_epilogue8<T>(epi, vec, C + m * ldc, m, sb, st, n0 + c, N, v);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its partial tile
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// CTAs of one cluster over K: as many as keep the grid within the SMs, at least two
+// slabs each, 1, 2, 4 or 8.
+inline int fp8_split(int64_t tiles, int64_t k_blocks) {
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= num_sms() && k_blocks >= 4 * split) split *= 2;
+  return split;
+}
+
+template <typename T>
+void launch_fp8_tile(const void* A, int64_t lda, const void* As, const void* W, int64_t ldw, const void* Ws, T* C,
+                     int64_t ldc, int64_t M, int64_t N, int64_t K, const Epi<T>& epi, bool vec, cudaStream_t s) {
+  using Cfg = Fp8TileCfg;
+  const uint64_t quads = uint64_t(fp8_quads(K));
+  const CUtensorMap ta = make_tmap_u8_2d(A, uint64_t(K), uint64_t(M), uint64_t(lda), 128);
+  const CUtensorMap tb = make_tmap_u8_2d(W, uint64_t(K), uint64_t(N), uint64_t(ldw), 128);
+  const CUtensorMap tsa = make_tmap_u32_2d(As, uint64_t(fp8_rows_padded(M)), quads, 128);
+  const CUtensorMap tsb = make_tmap_u32_2d(Ws, uint64_t(fp8_rows_padded(N)), quads, 128);
+  auto kern = gemm_fp8_tile_kernel<T>;
+  static std::atomic<uint64_t> smem_done{0};
+  ensure_smem_limit(smem_done, kern, Cfg::SMEM);
+  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
+  const int split = fp8_split(tiles, (K + 127) / 128);
+  LTX_UNSUPPORTED(tiles * split < (int64_t(1) << 31), "too many tiles for one launch");
+  launch_pdl(kern, dim3(unsigned(tiles * split)), dim3(192), Cfg::SMEM, s, unsigned(split), ta, tb, tsa, tsb, C, ldc,
+             int(M), int(N), int(K), split, int(vec), epi);
 }
 
 }  // namespace detail
@@ -440,12 +626,8 @@ extern "C" int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, 
     using T = std::remove_pointer_t<decltype(cp)>;
     bool vec;
     const Epi<T> e = make_epi_any<T>(epi, N, vec);
-    const dim3 grid{unsigned((N + 63) / 64), unsigned((M + 63) / 64)};
-    LTX_UNSUPPORTED(grid.y < 65536, "M too large");
-    linear_fp8_simt_kernel<T><<<grid, 256, 0, s>>>(
-        static_cast<const uint8_t*>(A), lda, static_cast<const uint32_t*>(a_scales), fp8_rows_padded(M),
-        static_cast<const uint8_t*>(W), ldw, static_cast<const uint32_t*>(w_scales), fp8_rows_padded(N), cp, ldc,
-        int(M), int(N), int(K), e), note_launch();
+    vec = vec && vec_ok(C, ldc);
+    launch_fp8_tile<T>(A, lda, a_scales, W, ldw, w_scales, cp, ldc, M, N, K, e, vec, s);
   };
   if (dtype == LTX_F32)
     run(static_cast<float*>(C));

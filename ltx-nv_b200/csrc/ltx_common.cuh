@@ -321,6 +321,60 @@ LTX_DEVICE void umma_commit(uint64_t* bar) {
                : "memory");
 }
 
+// Block-scaled 8-bit MMA (kind::mxf8f6f4, K = 32): both operands e4m3, K-major, every 32
+// values of a row multiplied by a power of two read from tensor memory at sfa / sfb (byte
+// a_sf / b_sf of the row's word, chosen by the instruction descriptor).
+LTX_DEVICE void umma_mx8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
+                            uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::
+          "r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+LTX_DEVICE void umma_mx8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                 uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::
+          "r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor of the block-scaled MMA: e4m3 operands, power-of-two (UE8M0)
+// scales, byte `sf` of the scale words for both operands.
+__host__ __device__ constexpr uint32_t umma_idesc_mx8(int M, int N, int sf) {
+  return (uint32_t(sf & 3) << 4)        // scale byte of B
+         | (uint32_t(N >> 3) << 17)     // N / 8
+         | (1u << 23)                   // scale format: UE8M0
+         | (uint32_t(M >> 4) << 24)     // M / 16
+         | (uint32_t(sf & 3) << 29);    // scale byte of A
+}
+// 32 rows of 16 bytes (512 contiguous bytes of shared memory) -> 4 columns of tensor
+// memory, repeated in the four 32-lane quadrants: the scale words of 128 operand rows.
+// Ordered with the MMAs of the same thread.
+LTX_DEVICE uint64_t umma_desc_rows16(uint32_t smem_addr) {
+  return uint64_t((smem_addr & 0x3FFFF) >> 4) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+LTX_DEVICE void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+LTX_DEVICE void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// 16 bytes of another CTA's shared memory, by its shared::cluster address.
+LTX_DEVICE float4 ld_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
+  return v;
+}
+
 // Instruction descriptor for kind::f16 with bf16 A/B, fp32 D, both operands K-major
 // unless b_mn_major is set (B stored with N contiguous).
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, int b_mn_major) {

@@ -29,6 +29,12 @@ CUtensorMap make_tmap_bf16_4d(const void* ptr, const uint64_t (&dims)[4], const 
                               const uint32_t (&box)[4]);
 CUtensorMap make_tmap_bf16_2d(const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner,
                               uint32_t box_outer);
+// Encode a 2-D, 128-byte-swizzled map over bytes (8-bit rows): inner bytes per row, outer
+// rows, ld bytes between rows (a multiple of 16), box of 128 bytes x box_outer rows.
+CUtensorMap make_tmap_u8_2d(const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_outer);
+// Encode an unswizzled 2-D map over a contiguous (outer, inner) array of 32-bit words, box
+// of box_inner words x 1 row.
+CUtensorMap make_tmap_u32_2d(const void* ptr, uint64_t inner, uint64_t outer, uint32_t box_inner);
 
 // Cache of encoded tensor maps, keyed by everything a 2-D map encodes (address,
 // extents, row stride, box), so a hit is always the descriptor a fresh encoding would

@@ -136,10 +136,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
-    """x (..., K) float32 or bfloat16 -> its (rows, K) matrix of 8-bit rows: e4m3 values with
-    a power-of-two scale per 128 columns. Weights (N, K) are quantised with it once."""
+    """x (..., K) float32 or bfloat16 -> its 8-bit rows: e4m3 values with a power-of-two scale
+    per 128 columns. Weights (N, K) are quantised with it once."""
     x2 = x.reshape(-1, x.shape[-1])
-    return nat.quantize_fp8(x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous())
+    return nat.quantize_fp8(x2 if x2.stride(1) == 1 else x2.contiguous(), x.shape)
 
 
 def _modulation(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None):
@@ -180,14 +180,13 @@ _NORM_KINDS = {"rms": nat.LTX_NORM_RMS, "layer": nat.LTX_NORM_LAYER, "none": nat
 
 def norm_modulate_fp8(x: torch.Tensor, scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
                       kind: str = "rms", eps: float = 1e-6) -> Fp8Rows:
-    """norm(x) * (1 + scale) + shift of x (B, T, D) as (B * T, D) 8-bit rows, the operand of
-    linear_fp8: fp32 arithmetic and one rounding. scale and shift (B, D) or (B, T, D) in x's
+    """norm(x) * (1 + scale) + shift of x (B, T, D) as 8-bit rows, the operand of linear_fp8: fp32 arithmetic and one rounding. scale and shift (B, D) or (B, T, D) in x's
     type; kind "rms", "layer" or "none"; D a multiple of 8."""
     if kind not in _NORM_KINDS:
         raise ValueError(f"kind must be one of {sorted(_NORM_KINDS)}, got {kind!r}")
     x2 = _row_major(x)
     mod, held = _modulation(x, shift, scale)
-    out = nat.norm_modulate_fp8(x2, max(x.shape[1], 1), _NORM_KINDS[kind], eps, mod)
+    out = nat.norm_modulate_fp8(x2, max(x.shape[1], 1), _NORM_KINDS[kind], eps, mod, x.shape)
     del held  # the vectors live until the launch; the allocator keeps stream order after it
     return out
 
@@ -201,11 +200,11 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
     """activation(x W^T + bias), or residual + gate * (x W^T + bias), with both operands in
     8-bit rows and fp32 sums, rounded once to `dtype`.
 
-    x: (..., K) float32 or bfloat16, quantised here (quantize_fp8), or its Fp8Rows already
-    (from norm_modulate_fp8). weight: (N, K) Fp8Rows. The result is (..., N), or (rows, N) /
-    residual's shape for an Fp8Rows x, in `dtype` (default: x's type, residual's, or
-    bfloat16). gate: (B, N) per sample or (B, T, N) per token of a (B, T, N) residual; bias,
-    residual and gate are in `dtype`. out may be the residual itself."""
+    x: (..., K) float32 or bfloat16, quantised here (quantize_fp8), or 8-bit rows already
+    (norm_modulate_fp8). weight: (N, K) Fp8Rows. The result is (..., N) in `dtype` (default:
+    x's type; for 8-bit rows the residual's, or bfloat16). gate: (B, N) per sample or (B, T,
+    N) per token of a (B, T, N) result; bias, residual and gate are in `dtype`. out may be the
+    residual itself."""
     if not isinstance(weight, Fp8Rows):
         raise TypeError("weight must be Fp8Rows (quantize_fp8 or Fp8Rows.from_parts)")
     if activation not in _ACTIVATIONS:
@@ -215,18 +214,12 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
     if activation is not None and residual is not None:
         raise ValueError("an activation and a residual exclude each other")
     n = weight.rows
-    if isinstance(x, Fp8Rows):
-        lead = tuple(residual.shape[:-1]) if residual is not None else \
-            tuple(out.shape[:-1]) if out is not None else (x.rows,)
-        dtype = dtype or (residual.dtype if residual is not None else out.dtype if out is not None else torch.bfloat16)
-        cols = x.cols
-    else:
-        lead, dtype, cols = tuple(x.shape[:-1]), dtype or x.dtype, x.shape[-1]
-    if cols != weight.cols:
-        raise ValueError(f"x has {cols} columns, the weight {weight.cols}")
+    if dtype is None:
+        dtype = x.dtype if isinstance(x, torch.Tensor) else residual.dtype if residual is not None else torch.bfloat16
+    if x.shape[-1] != weight.cols or len(weight.shape) != 2:
+        raise ValueError(f"x has {x.shape[-1]} columns, the weight is {weight.shape}")
+    lead = tuple(x.shape[:-1])
     shape = (*lead, n)
-    if isinstance(x, Fp8Rows) and math.prod(lead) != x.rows:
-        raise ValueError(f"{x.rows} rows do not fill {shape}")
     for name, t, want in (("bias", bias, (n,)), ("residual", residual, shape), ("out", out, shape)):
         if t is not None and (tuple(t.shape) != want or t.dtype != dtype or t.device != x.device):
             raise ValueError(f"{name} must be {dtype} {want} on {x.device}, got {t.dtype} {tuple(t.shape)}")

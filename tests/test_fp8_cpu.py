@@ -31,7 +31,7 @@ def test_scale_bytes(lib):
     assert lib.ltx_fp8_scale_bytes(256, 512) == 256 * 4
     assert lib.ltx_fp8_scale_bytes(257, 513) == 512 * 2 * 4
     assert lib.ltx_fp8_scale_bytes(0, 5) == 0 and lib.ltx_fp8_scale_bytes(5, -1) == 0
-    r = nat.Fp8Rows(257, 513, "cpu")
+    r = nat.Fp8Rows(257, 513, device="cpu")
     assert r.scales.numel() * 4 == lib.ltx_fp8_scale_bytes(257, 513)
     assert r.data.shape == (257, 513) and r.data.stride(0) == 528
 
@@ -99,7 +99,7 @@ def test_masked_attention_refusals(lib, change, status):
 
 def test_python_entry_points_refuse_bad_arguments():
     x = torch.zeros(2, 3, 256, dtype=torch.bfloat16)
-    w = nat.Fp8Rows(64, 256, "cpu")
+    w = nat.Fp8Rows(64, 256, device="cpu")
     with pytest.raises(ValueError, match="CUDA"):
         ltx_nn.quantize_fp8(x)
     with pytest.raises(TypeError):
@@ -123,8 +123,8 @@ def test_python_entry_points_refuse_bad_arguments():
         ltx_nn.linear_fp8(x, w, bias=torch.zeros(63, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="contiguous"):
         ltx_nn.linear_fp8(x, w, out=torch.zeros(2, 64, 3, dtype=torch.bfloat16).transpose(1, 2))
-    with pytest.raises(ValueError, match="do not fill"):
-        ltx_nn.linear_fp8(nat.Fp8Rows(7, 256, "cpu"), w, residual=res)
+    with pytest.raises(ValueError, match="residual must"):
+        ltx_nn.linear_fp8(nat.Fp8Rows(7, 256, device="cpu"), w, residual=res)
     with pytest.raises(ValueError, match="kind"):
         ltx_nn.norm_modulate_fp8(x, kind="batch")
     with pytest.raises(ValueError, match="scale must"):

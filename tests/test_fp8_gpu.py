@@ -142,7 +142,8 @@ def test_norm_modulate_fp8(b, t, d, per_token, dtype, kind):
         got = ltx_nn.norm_modulate_fp8(x, scale=scale, shift=shift, kind=kind, eps=1e-6)
         y = ref.norm_modulate(x, scale, shift, kind, 1e-6).reshape(b * t, d)
         want, s = ref.quantize(y)
-        v = got.dequantize(torch.float32).double().cpu()
+        assert got.shape == (b, t, d)
+        v = got.dequantize(torch.float32).double().cpu().view(b * t, d)
         step = torch.maximum(want.abs() * 2.0 ** -3, s.repeat_interleave(128, 1)[:, :d] * 2.0 ** -9)
         assert ((v - want).abs() <= 2 * step).all()
         # a tie within eps of y: probability about 2 eps / step-to-magnitude 2^-4, times 4 for
@@ -166,6 +167,7 @@ def test_norm_modulate_fp8_takes_slices_of_an_adaln_output():
     y = ref.norm_modulate(x, mod[:, d:2 * d].double() + table[1].double(), mod[:, :d].double() + table[0].double(),
                           "rms", 1e-6)
     want, _ = ref.quantize(y.reshape(-1, d))
+    assert torch.equal(got.data.float(), nat.norm_modulate_fp8(x.view(-1, d), t, 0, 1e-6, m, (b, t, d)).data.float())
     v = got.dequantize(torch.float32).double().cpu()
     assert (v != want).double().mean() <= 8 * (d + 8) * 2.0 ** -24 * 2 ** 4
 
