@@ -7,6 +7,8 @@
 // of the type's lowest finite value (the "lowest value" and -inf conventions alike);
 // what K and V hold at such a key (NaN and infinities included) does not reach any
 // output. A row whose keys are all left out, or whose scores are all -inf, is zero.
+#include <algorithm>
+
 #include "ltx_kernels.cuh"
 
 namespace ltx {
@@ -94,6 +96,636 @@ __global__ void __launch_bounds__(128) masked_attn_simt_kernel(const T* __restri
   for (int c = 0; c < D; ++c) st_elem<T>(op + c, acc[c] * inv);
 }
 
+// ---------------------------------------------------------------------------------
+// bf16: persistent tcgen05 kernel. A unit is (sample, head, 256 queries) = two 128-row Q
+// tiles; CTAs walk the units in steps of the grid, and every role runs straight on from
+// one unit to the next, so a unit's Q load, first Q K^T and output store overlap its
+// neighbours' softmax: with the few key tiles of a text context, the fixed cost of a
+// unit would otherwise be as large as its work.
+//   warps 0-3, 4-7  softmax of Q tile 0 / 1 (one query row per thread = TMEM lane)
+//   warp 8          reads a sample's mask into the list of its key tiles (128 keys each) that
+//                   hold any key, loads Q and the listed K / V tiles by TMA, and leaves a
+//                   descriptor (MaTile) beside each stage that the other roles follow
+//   warps 9, 10     MMA issuers of Q tile 0 / 1 (head_dim 128: warp 9 issues both)
+//   warp 11         tiles that need more than plain scores: what each key adds to them (-inf:
+//                   left out) in shared memory, and V rows of left-out keys set to zero, so
+//                   that no NaN there can reach P V (0 * NaN)
+// Tiles without a key are never loaded; plain tiles run the unmasked softmax (packed
+// arithmetic, part of the exponentials on the FMA pipe, lazy rescaling: attention.cu).
+// TMEM as in attention.cu: head_dim 64 keeps P beside S (S_i is computed two tiles
+// ahead), head_dim 128 writes P over S.
+// split > 1 (few units, many key tiles): the CTAs of a cluster take shares of one unit's
+// list and merge their fp32 O / l and log-sum-exp through distributed shared memory, in
+// rank order.
+// ---------------------------------------------------------------------------------
+template <int D>
+struct MaCfg {
+  static constexpr int SUB = D / 64;              // 64-column (128-byte) sub-tiles per row
+  static constexpr int TILE = 128 * D * 2;        // one Q, K or V tile
+  static constexpr bool SEP_P = D == 64;          // P in its own TMEM columns
+  static constexpr int STAGES = SEP_P ? 4 : 2;    // K / V ring
+  static constexpr int QBUF = SEP_P ? 2 : 1;      // units whose Q is in shared memory
+  static constexpr int ISSUERS = SEP_P ? 2 : 1;
+  static constexpr int MAX_TILES = 4096;          // list entries: Tk <= 524288
+  static constexpr int RING = TILE * 2 * (QBUF + STAGES);
+  static constexpr int BIAS = STAGES * 128 * 4;
+  static constexpr int LIST = MAX_TILES * 2;
+  static constexpr int SMEM = RING + BIAS + LIST + 512 + 1024;
+  static constexpr int LD_PART = D + 4;           // floats per row of a split unit's partial
+  static_assert(256 * LD_PART * 4 + 256 * 4 <= RING, "the partial reuses the operand ring");
+  static_assert((2 * QBUF + 4 * STAGES + 8) * 8 + STAGES * 16 + 8 <= 512, "barriers and descriptors");
+  static constexpr uint32_t s_col(int i) { return uint32_t(128 * i); }
+  static constexpr uint32_t p_col(int i) { return SEP_P ? uint32_t(256 + 64 * i) : uint32_t(128 * i); }
+  static constexpr uint32_t o_col(int i) { return SEP_P ? uint32_t(384 + 64 * i) : uint32_t(256 + D * i); }
+};
+
+struct MaParams {
+  int H, Tq, Tk, nq2;
+  int units, split;  // split: CTAs of a cluster that share a unit
+  float scale_log2;
+  KeyMask mask;
+  const __nv_bfloat16* gate;
+  int64_t ld_gate;
+  __nv_bfloat16* O;
+  int64_t ldo;
+
+  LTX_DEVICE int sample(int u) const { return u / (nq2 * H); }
+  LTX_DEVICE int head(int u) const { return (u / nq2) % H; }
+  LTX_DEVICE int q0(int u) const { return (u % nq2) * 256; }
+};
+
+// What a K / V stage holds: a key tile of a unit. FIRST / LAST of the unit's tiles; MARKED:
+// its scores need sbias; TWO: Q tile 1 of the unit has rows; END: no more tiles.
+struct MaTile {
+  int unit, tile, flags, pad;
+};
+enum : int { MA_FIRST = 1, MA_LAST = 2, MA_MARKED = 4, MA_TWO = 8, MA_END = 16 };
+
+LTX_DEVICE void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    masked_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                          const __grid_constant__ CUtensorMap tmV, const MaParams P) {
+  using Cfg = MaCfg<D>;
+  constexpr int S = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = fa_align1024(smem_raw);
+  uint8_t* sQ = smem;                               // unit buffer k, Q tile i at (2k + i) * TILE
+  uint8_t* sKV = smem + 2 * Cfg::QBUF * Cfg::TILE;  // stage s: K at 2s * TILE, V behind it
+  float* sbias = reinterpret_cast<float*>(smem + Cfg::RING);  // [S][128], log2 units
+  uint16_t* list = reinterpret_cast<uint16_t*>(smem + Cfg::RING + Cfg::BIAS);  // warp 8's
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::RING + Cfg::BIAS + Cfg::LIST);
+  uint64_t* q_full = bars;                   // [QBUF]
+  uint64_t* q_empty = q_full + Cfg::QBUF;    // [QBUF]
+  uint64_t* k_full = q_empty + Cfg::QBUF;    // [S] descriptor and K
+  uint64_t* v_full = k_full + S;             // [S]
+  uint64_t* v_fix = v_full + S;              // [S] V and bias ready (warp 11)
+  uint64_t* kv_empty = v_fix + S;            // [S] both Q tiles' P V done
+  uint64_t* s_full = kv_empty + S;           // [2]
+  uint64_t* s_free = s_full + 2;             // [2] SEP_P only
+  uint64_t* p_full = s_free + 2;             // [2]
+  uint64_t* o_done = p_full + 2;             // [2]
+  MaTile* desc = reinterpret_cast<MaTile*>(o_done + 2);  // [S]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(desc + S);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = lane_id();
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < Cfg::QBUF; ++k) {
+      mbar_init(&q_full[k], 1);
+      mbar_init(&q_empty[k], Cfg::ISSUERS);
+    }
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_fix[s], 1);
+      mbar_init(&kv_empty[s], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 128);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  // this CTA's units, and its share of each unit's list
+  const int u0 = int(blockIdx.x) / P.split, rank = int(blockIdx.x) - u0 * P.split;
+  const int u_step = P.split > 1 ? P.units : int(gridDim.x);
+  // softmax state of a split unit, for the merge
+  float m_ref = -INFINITY, l_run = 0.f;
+  bool have = false;
+
+  if (warp == 8) {
+    // ------------------------- lists and TMA producer -------------------------
+    const int n_tiles = (P.Tk + 127) / 128;
+    if (lane == 0) {
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    int b = -1, lo = 0, n = 0, g = 0, un = 0;
+    bool ok = true;
+    for (int u = u0; ok && u < P.units; u += u_step) {
+      const int nb = P.sample(u), h = P.head(u), q0 = P.q0(u);
+      if (nb != b) {
+        b = nb;
+        int count = 0;
+        __syncwarp();
+        for (int t0 = 0; t0 < n_tiles; t0 += 32) {
+          uint32_t any = 0, plain = 0;  // bit j: tile t0 + j
+          const int nt = min(32, n_tiles - t0);
+#pragma unroll 4
+          for (int j = 0; j < nt; ++j) {
+            const int key = (t0 + j) * 128 + lane;
+            bool a = false, p = true;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float v = key + 32 * c < P.Tk ? P.mask.at(b, key + 32 * c) : -INFINITY;
+              a |= v != -INFINITY;
+              p &= v == 0.f;
+            }
+            if (__any_sync(0xffffffffu, a)) any |= 1u << j;
+            if (__all_sync(0xffffffffu, p)) plain |= 1u << j;
+          }
+          if ((any >> lane) & 1u)
+            list[count + __popc(any & ((1u << lane) - 1u))] =
+                uint16_t((t0 + lane) | (((plain >> lane) & 1u) ? 0 : 0x8000));
+          count += __popc(any);
+        }
+        __syncwarp();
+        lo = int(int64_t(count) * rank / P.split);
+        n = int(int64_t(count) * (rank + 1) / P.split) - lo;
+      }
+      if (n == 0) {
+        if (P.split == 1) {  // no key: zero rows
+          constexpr int LPR = D / 8;  // lanes per row, 16 bytes each
+          for (int r = lane / LPR; r < min(256, P.Tq - q0); r += 32 / LPR)
+            *reinterpret_cast<uint4*>(P.O + (int64_t(b) * P.Tq + q0 + r) * P.ldo + int64_t(h) * D + (lane % LPR) * 8) =
+                make_uint4(0, 0, 0, 0);
+        }
+        continue;
+      }
+      if (lane == 0) {
+        const int k = un % Cfg::QBUF, col0 = h * D, two = q0 + 128 < P.Tq ? 1 : 0;
+        ok = mbar_wait(&q_empty[k], (uint32_t(un / Cfg::QBUF) & 1) ^ 1, abort_flag);
+        if (ok) {
+          mbar_arrive_expect_tx(&q_full[k], (1 + two) * Cfg::TILE);
+          for (int i = 0; i <= two; ++i)
+#pragma unroll
+            for (int j = 0; j < Cfg::SUB; ++j)
+              tma_load_2d(sQ + (2 * k + i) * Cfg::TILE + j * 16384, &tmQ, &q_full[k], col0 + 64 * j,
+                          b * P.Tq + q0 + i * 128);
+        }
+        for (int t = 0; ok && t < n; ++t, ++g) {
+          const int s = g % S;
+          ok = mbar_wait(&kv_empty[s], (uint32_t(g / S) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          const int e = list[lo + t], tile = e & 0x7fff;
+          desc[s] = MaTile{u, tile, (t == 0 ? MA_FIRST : 0) | (t == n - 1 ? MA_LAST : 0) |
+                                       ((e & 0x8000) ? MA_MARKED : 0) | (two ? MA_TWO : 0), 0};
+          uint8_t* sk = sKV + 2 * s * Cfg::TILE;
+          const int row = b * P.Tk + tile * 128;
+          mbar_arrive_expect_tx(&k_full[s], Cfg::TILE);
+#pragma unroll
+          for (int j = 0; j < Cfg::SUB; ++j) tma_load_2d(sk + j * 16384, &tmK, &k_full[s], col0 + 64 * j, row);
+          mbar_arrive_expect_tx(&v_full[s], Cfg::TILE);
+#pragma unroll
+          for (int j = 0; j < Cfg::SUB; ++j)
+            tma_load_2d(sk + Cfg::TILE + j * 16384, &tmV, &v_full[s], col0 + 64 * j, row);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+      ++un;
+    }
+    if (lane == 0 && ok && mbar_wait(&kv_empty[g % S], (uint32_t(g / S) & 1) ^ 1, abort_flag)) {
+      desc[g % S] = MaTile{0, 0, MA_END, 0};
+      mbar_arrive(&k_full[g % S]);
+    }
+  } else if (warp == 9 || warp == 10) {
+    // ------------------------------ MMA issuers ------------------------------
+    constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0);
+    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
+    // Scores of tile g for Q tile i (k: the unit's Q buffer). A unit without a Q tile 1 has
+    // no MMAs there; its barriers advance all the same, so every phase is the tile's number.
+    auto issue_qk = [&](int i, int g, int k, int flags) {
+      if (i == 0 || (flags & MA_TWO)) {
+        const uint32_t qa = smem_u32(sQ) + uint32_t((2 * k + i) * Cfg::TILE);
+        const uint32_t ka = smem_u32(sKV + 2 * (g % S) * Cfg::TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = uint32_t((kk >> 2) * 16384 + (kk & 3) * 32);
+          umma_ss(tmem + Cfg::s_col(i), umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
+                  idesc_s, kk > 0 ? 1u : 0u);
+        }
+      }
+      umma_commit(&s_full[i]);
+    };
+    auto issue_pv = [&](int i, int g, int flags) {
+      if (i == 0 || (flags & MA_TWO)) {
+        const uint32_t va = smem_u32(sKV + (2 * (g % S) + 1) * Cfg::TILE);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(tmem + Cfg::o_col(i), tmem + Cfg::p_col(i) + uint32_t(kk * 8),
+                  umma_desc_sw128(va + uint32_t(kk * 2048), 16384, 1024), idesc_o,
+                  (!(flags & MA_FIRST) || kk > 0) ? 1u : 0u);
+      }
+      umma_commit(&o_done[i]);
+      umma_commit(&kv_empty[g % S]);  // count 2: both Q tiles' P V of this stage
+    };
+    auto wait_k = [&](int g) { return mbar_wait(&k_full[g % S], uint32_t(g / S) & 1, abort_flag); };
+    auto wait_q = [&](int un) {
+      return mbar_wait(&q_full[un % Cfg::QBUF], uint32_t(un / Cfg::QBUF) & 1, abort_flag);
+    };
+    if (lane == 0 && warp - 9 < Cfg::ISSUERS) {
+      int gq = 0, un = 0;  // next tile whose scores are issued, and its unit
+      bool more = true;    // no END seen yet
+      if constexpr (Cfg::SEP_P) {
+        // Q tile i: P_i V_g, then Q_i K_{g+2}^T (attention.cu).
+        const int i = warp - 9;
+        auto qk_step = [&]() {
+          if (!wait_k(gq)) return false;
+          const int flags = desc[gq % S].flags;
+          if (flags & MA_END) {
+            more = false;
+            return true;
+          }
+          if ((flags & MA_FIRST) && !wait_q(un)) return false;
+          if (gq > 0 && !mbar_wait(&s_free[i], uint32_t(gq - 1) & 1, abort_flag)) return false;
+          tc_fence_after();
+          issue_qk(i, gq, un % Cfg::QBUF, flags);
+          if (flags & MA_LAST) umma_commit(&q_empty[un++ % Cfg::QBUF]);
+          ++gq;
+          return true;
+        };
+        bool ok = qk_step() && (!more || qk_step());
+        for (int g = 0; ok && g < gq; ++g) {
+          const int s = g % S, flags = desc[s].flags;
+          ok = mbar_wait(&v_fix[s], uint32_t(g / S) & 1, abort_flag) &&
+               mbar_wait(&p_full[i], uint32_t(g) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(i, g, flags);
+          if (more) ok = qk_step();
+        }
+      } else {
+        // Both Q tiles: P_0 V_g, Q_0 K_{g+1}^T, P_1 V_g, Q_1 K_{g+1}^T (attention.cu).
+        bool ok = wait_k(0);
+        int flags = ok ? desc[0].flags : MA_END;
+        if (ok && !(flags & MA_END)) {
+          ok = wait_q(0);
+          if (ok) {
+            tc_fence_after();
+            issue_qk(0, 0, 0, flags);
+            issue_qk(1, 0, 0, flags);
+            if (flags & MA_LAST) umma_commit(&q_empty[0]), ++un;
+          }
+        }
+        for (int g = 0; ok && !(flags & MA_END); ++g) {
+          ok = mbar_wait(&v_fix[g % S], uint32_t(g / S) & 1, abort_flag);
+          int next = MA_END;
+          for (int i = 0; ok && i < 2; ++i) {
+            if (!mbar_wait(&p_full[i], uint32_t(g) & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            issue_pv(i, g, flags);
+            if (i == 0) {  // the next tile's K (and Q), awaited behind the first P V
+              ok = wait_k(g + 1);
+              if (!ok) break;
+              next = desc[(g + 1) % S].flags;
+              if ((next & MA_FIRST) && !(ok = wait_q(un))) break;
+              tc_fence_after();
+            }
+            if (!(next & MA_END)) {
+              issue_qk(i, g + 1, un % Cfg::QBUF, next);
+              if (i == 1 && (next & MA_LAST)) umma_commit(&q_empty[un++ % Cfg::QBUF]);
+            }
+          }
+          flags = next;
+        }
+      }
+    }
+  } else if (warp == 11) {
+    // ------------------------- marked tiles: bias and V -------------------------
+    for (int g = 0;; ++g) {
+      const int s = g % S;
+      const uint32_t par = uint32_t(g / S) & 1;
+      if (!mbar_wait(&k_full[s], par, abort_flag)) break;
+      const MaTile d = desc[s];
+      if (d.flags & MA_END) break;
+      float v[4];
+      uint32_t keep[4];
+      if (d.flags & MA_MARKED) {
+        const int b = P.sample(d.unit);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int key = d.tile * 128 + 32 * c + lane;
+          v[c] = key < P.Tk ? P.mask.at(b, key) : -INFINITY;
+        }
+      }
+      if (!mbar_wait(&v_full[s], par, abort_flag)) break;
+      if (d.flags & MA_MARKED) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          sbias[s * 128 + 32 * c + lane] = v[c] * 1.4426950408889634f;
+          keep[c] = __ballot_sync(0xffffffffu, v[c] != -INFINITY);
+        }
+        uint8_t* sv = sKV + (2 * s + 1) * Cfg::TILE + (lane >> 3) * 128 + (lane & 7) * 16;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int r = 0; r < 32; r += 4) {
+            if (!((keep[c] >> (r + (lane >> 3))) & 1u)) {
+#pragma unroll
+              for (int j = 0; j < Cfg::SUB; ++j)
+                *reinterpret_cast<uint4*>(sv + j * 16384 + (32 * c + r) * 128) = make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(&v_fix[s]);
+    }
+  } else {
+    // --------------------- softmax / correction / epilogue ---------------------
+    const int qt = warp >> 2;                // Q tile of this warpgroup
+    const int row = (warp & 3) * 32 + lane;  // row within the tile == TMEM lane
+    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + Cfg::s_col(qt) + lane_off;
+    const uint32_t p_tmem = tmem + Cfg::p_col(qt) + lane_off;
+    const uint32_t o_tmem = tmem + Cfg::o_col(qt) + lane_off;
+    for (int g = 0;; ++g) {
+      const int s = g % S;
+      if (!mbar_wait(&k_full[s], uint32_t(g / S) & 1, abort_flag)) break;
+      const int flags = desc[s].flags;
+      if (flags & MA_END) break;
+      if (!mbar_wait(&s_full[qt], uint32_t(g) & 1, abort_flag)) break;
+      if (qt == 1 && !(flags & MA_TWO)) {
+        if (Cfg::SEP_P) mbar_arrive(&s_free[qt]);
+        // one p_full phase ahead of the issuer at most, as below
+        if (g > 0 && !mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
+        mbar_arrive(&p_full[qt]);
+        continue;
+      }
+      const int unit = desc[s].unit;  // the stage may be refilled once P is handed over
+      const bool first = flags & MA_FIRST;
+      tc_fence_after();
+      float sv[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + uint32_t(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&sv[c * 32]));
+      tmem_wait_ld();
+      if constexpr (Cfg::SEP_P) {
+        tc_fence_before();
+        mbar_arrive(&s_free[qt]);
+      }
+      float sc = P.scale_log2;
+      const bool marked = flags & MA_MARKED;
+      if (marked) {
+        // scores in log2 units with the mask added; a left-out key's is -inf whatever K held
+        if (!mbar_wait(&v_fix[s], uint32_t(g / S) & 1, abort_flag)) break;
+        const float4* bias = reinterpret_cast<const float4*>(sbias + s * 128);
+#pragma unroll
+        for (int e = 0; e < 128; e += 4) {
+          const float4 bb = bias[e >> 2];
+          sv[e] = bb.x == -INFINITY ? -INFINITY : fmaf(sv[e], sc, bb.x);
+          sv[e + 1] = bb.y == -INFINITY ? -INFINITY : fmaf(sv[e + 1], sc, bb.y);
+          sv[e + 2] = bb.z == -INFINITY ? -INFINITY : fmaf(sv[e + 2], sc, bb.z);
+          sv[e + 3] = bb.w == -INFINITY ? -INFINITY : fmaf(sv[e + 3], sc, bb.w);
+        }
+        sc = 1.f;
+      }
+      float m8[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m8[e] = sv[e];
+#pragma unroll
+      for (int e = 8; e < 128; e += 16)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
+      const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+      const float m_cand = mx * sc;
+      if (first) {
+        m_ref = -INFINITY;
+        l_run = 0.f;
+      }
+      const bool need = first || (m_cand > m_ref + 8.f);
+      float alpha = 1.f;
+      if (need) {
+        const float m_new = fmaxf(m_ref, m_cand);
+        alpha = first || m_new == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
+        m_ref = m_new;
+      }
+      const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;  // a row of -inf so far: weights 0
+      const uint64_t sc2 = f2_pack(sc, sc);
+      const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
+      uint64_t rs2[4] = {0, 0, 0, 0};
+      uint32_t pk[64];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float x0, x1, p0, p1;
+          f2_unpack(f2_fma(f2_pack(sv[c * 32 + e], sv[c * 32 + e + 1]), sc2, nm2), x0, x1);
+          if (!marked && ((kFaPolyPairs >> (c * 16 + (e >> 1))) & 1u)) {
+            ex2_poly2(x0, x1, p0, p1);
+          } else {
+            p0 = ex2_approx(x0);
+            p1 = ex2_approx(x1);
+          }
+          rs2[(e >> 1) & 3] = f2_add(rs2[(e >> 1) & 3], f2_pack(p0, p1));
+          pk[c * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
+        }
+        if constexpr (!Cfg::SEP_P) tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
+      }
+      if constexpr (Cfg::SEP_P) {
+        // P_i V_{g-1} has read P_i, and the issuer has seen p_full of tile g - 1
+        if (g > 0) {
+          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
+      }
+      float r0, r1;
+      f2_unpack(f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3])), r0, r1);
+      if (!first && __any_sync(0xffffffffu, need)) {
+        if (!Cfg::SEP_P) {
+          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t rr[32];
+          tmem_ld32(o_tmem + uint32_t(c0), rr);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) rr[e] = __float_as_uint(__uint_as_float(rr[e]) * alpha);
+          tmem_st32(o_tmem + uint32_t(c0), rr);
+        }
+      }
+      l_run = l_run * alpha + (r0 + r1);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[qt]);
+      if (!(flags & MA_LAST)) continue;
+      // ------------------------- the unit's output rows -------------------------
+      if (!mbar_wait(&o_done[qt], uint32_t(g) & 1, abort_flag)) break;
+      tc_fence_after();
+      if (P.split > 1) {
+        have = true;
+        continue;  // the END descriptor follows
+      }
+      const int b = P.sample(unit), h = P.head(unit);
+      const int qi = P.q0(unit) + qt * 128 + row;
+      const bool live = qi < P.Tq;
+      const int64_t orow = int64_t(b) * P.Tq + qi;
+      float f = l_run == 0.f ? 0.f : 1.f / l_run;
+      if (P.gate != nullptr && live) f *= 2.f / (1.f + __expf(-__bfloat162float(P.gate[orow * P.ld_gate + h])));
+      __nv_bfloat16* op = P.O + orow * P.ldo + int64_t(h) * D;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t rr[32];
+        tmem_ld32(o_tmem + uint32_t(c0), rr);
+        tmem_wait_ld();
+        if (live) {
+#pragma unroll
+          for (int e8 = 0; e8 < 32; e8 += 8) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(rr[e8 + e]) * f;
+            st8<__nv_bfloat16>(op + c0 + e8, v);
+          }
+        }
+      }
+    }
+    if (P.split > 1) {
+      // fp32 O / l and the row's log2-sum-exp of this share, in the operand ring (every P V of
+      // both Q tiles has completed once all eight warps are here)
+      named_bar_sync(1, 256);
+      float* part = reinterpret_cast<float*>(smem);
+      float* lse = part + 256 * Cfg::LD_PART;
+      const int r = qt * 128 + row;
+      const bool some = have && l_run != 0.f;
+      if (have) {
+        const float inv = some ? 1.f / l_run : 0.f;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t rr[32];
+          tmem_ld32(o_tmem + uint32_t(c0), rr);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(part + r * Cfg::LD_PART + c0 + e) =
+                make_float4(__uint_as_float(rr[e]) * inv, __uint_as_float(rr[e + 1]) * inv,
+                            __uint_as_float(rr[e + 2]) * inv, __uint_as_float(rr[e + 3]) * inv);
+        }
+      }
+      lse[r] = some ? m_ref + log2f(l_run) : -INFINITY;
+    }
+  }
+  __syncwarp();
+  if (P.split > 1) {
+    cluster_sync_all();
+    const int u = u0, b = P.sample(u), h = P.head(u), q0 = P.q0(u);
+    const int rows = min(256, P.Tq - q0);
+    constexpr int C8 = D / 8;
+    const uint32_t base = smem_u32(smem);
+    // the ranks take the row pieces of 8 columns in turn
+    for (int i = int(threadIdx.x) * P.split + rank; i < rows * C8; i += 384 * P.split) {
+      const int r = i / C8, c = (i - r * C8) * 8;
+      const uint32_t at_l = base + uint32_t(256 * Cfg::LD_PART + r) * 4u;
+      const uint32_t at_o = base + uint32_t(r * Cfg::LD_PART + c) * 4u;
+      float top = -INFINITY, sum = 0.f, v[8] = {};
+      float wl[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        wl[p] = p < P.split ? ld_cluster_f1(mapa_shared(at_l, uint32_t(p))) : -INFINITY;
+        top = fmaxf(top, wl[p]);
+      }
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        if (p < P.split && wl[p] != -INFINITY) {
+          const float wp = exp2f(wl[p] - top);
+          const uint32_t a = mapa_shared(at_o, uint32_t(p));
+          const float4 x = ld_cluster_f4(a), y = ld_cluster_f4(a + 16);
+          sum += wp;
+          v[0] += wp * x.x; v[1] += wp * x.y; v[2] += wp * x.z; v[3] += wp * x.w;
+          v[4] += wp * y.x; v[5] += wp * y.y; v[6] += wp * y.z; v[7] += wp * y.w;
+        }
+      }
+      const int64_t orow = int64_t(b) * P.Tq + q0 + r;
+      float f = sum == 0.f ? 0.f : 1.f / sum;
+      if (P.gate != nullptr) f *= 2.f / (1.f + __expf(-__bfloat162float(P.gate[orow * P.ld_gate + h])));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= f;
+      st8<__nv_bfloat16>(P.O + orow * P.ldo + int64_t(h) * D + c, v);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its part
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// CTAs of a cluster per unit: as many as keep the grid within the SMs, at least two key
+// tiles each, 1, 2, 4 or 8.
+inline int ma_split(int64_t units, int64_t Tk) {
+  int split = 1;
+  while (split < 8 && units * split * 2 <= num_sms() && Tk >= 128 * 4 * split) split *= 2;
+  return split;
+}
+
+template <int D>
+void launch_masked_tc(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
+                      int64_t ldo, int B, int64_t Tq, int64_t Tk, int H, float scale, const KeyMask& mask,
+                      const void* gate, int64_t ld_gate, cudaStream_t s) {
+  using Cfg = MaCfg<D>;
+  LTX_UNSUPPORTED(Tk <= int64_t(Cfg::MAX_TILES) * 128, "at most 524288 keys under a mask");
+  const uint64_t cols = uint64_t(H) * D;
+  const CUtensorMap tq = make_tmap_bf16_2d(q, cols, uint64_t(B) * Tq, uint64_t(ldq), 64, 128);
+  const CUtensorMap tk = make_tmap_bf16_2d(k, cols, uint64_t(B) * Tk, uint64_t(ldk), 64, 128);
+  const CUtensorMap tv = make_tmap_bf16_2d(v, cols, uint64_t(B) * Tk, uint64_t(ldv), 64, 128);
+  auto kern = masked_attn_tc_kernel<D>;
+  static std::atomic<uint64_t> smem_done{0};
+  ensure_smem_limit(smem_done, kern, Cfg::SMEM);
+  MaParams p{};
+  p.H = H;
+  p.Tq = int(Tq);
+  p.Tk = int(Tk);
+  p.nq2 = int((Tq + 255) / 256);
+  const int64_t units = int64_t(B) * H * p.nq2;
+  LTX_UNSUPPORTED(units < (int64_t(1) << 31) - 65536, "too many queries for one launch");
+  p.units = int(units);
+  p.split = ma_split(units, Tk);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.mask = mask;
+  p.gate = static_cast<const __nv_bfloat16*>(gate);
+  p.ld_gate = ld_gate;
+  p.O = static_cast<__nv_bfloat16*>(o);
+  p.ldo = ldo;
+  const int64_t grid = p.split > 1 ? units * p.split : std::min<int64_t>(units, num_sms());
+  launch_pdl(kern, dim3(unsigned(grid)), dim3(384), Cfg::SMEM, s, unsigned(p.split), tq, tk, tv, p);
+}
+
 }  // namespace detail
 }  // namespace ltx
 
@@ -142,12 +774,10 @@ extern "C" int ltx_attention_masked(const void* q, int64_t ldq, const void* k, i
       run(qp, std::integral_constant<int, 64>{});
     else
       run(qp, std::integral_constant<int, 128>{});
+  } else if (head_dim == 64) {
+    launch_masked_tc<64>(q, ldq, k, ldk, v, ldv, o, ldo, B, Tq, Tk, heads, scale, km, gate_logits, ld_gate, s);
   } else {
-    auto qp = static_cast<const __nv_bfloat16*>(q);
-    if (head_dim == 64)
-      run(qp, std::integral_constant<int, 64>{});
-    else
-      run(qp, std::integral_constant<int, 128>{});
+    launch_masked_tc<128>(q, ldq, k, ldk, v, ldv, o, ldo, B, Tq, Tk, heads, scale, km, gate_logits, ld_gate, s);
   }
   LTX_CUDA(cudaGetLastError());
   LTX_API_END

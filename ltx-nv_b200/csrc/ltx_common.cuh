@@ -365,7 +365,12 @@ LTX_DEVICE void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
 LTX_DEVICE void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-// 16 bytes of another CTA's shared memory, by its shared::cluster address.
+// 4 and 16 bytes of another CTA's shared memory, by its shared::cluster address.
+LTX_DEVICE float ld_cluster_f1(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 LTX_DEVICE float4 ld_cluster_f4(uint32_t cluster_addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"

@@ -78,7 +78,9 @@ def check(got, q, k, v, heads, left_out, bias, gate, scale):
 SHAPES = [(1, 1, 1, 1, 64), (2, 1, 7, 2, 128), (1, 3, 128, 4, 64), (2, 5, 129, 3, 64), (3, 126, 250, 4, 64),
           (2, 128, 127, 2, 128), (1, 129, 256, 2, 64), (2, 255, 384, 2, 128), (1, 256, 640, 4, 64), (1, 300, 1024, 2, 64),
           (4, 257, 1000, 2, 128), (2, 1, 4099, 4, 128), (3, 2, 2048, 5, 64), (2, 16, 513, 8, 64), (1, 17, 1300, 3, 128),
-          (2, 700, 77, 5, 64), (1, 513, 130, 20, 128), (1, 64, 5000, 2, 64)]
+          (2, 700, 77, 5, 64), (1, 513, 130, 20, 128), (1, 64, 5000, 2, 64),
+          # more units than SMs, every second one with rows in one of its two query tiles only
+          (4, 300, 200, 40, 64), (4, 270, 140, 40, 128), (40, 30, 260, 5, 64)]
 
 
 @pytest.mark.parametrize("kind", ["left", "right", "holes", "sparse", "all", "one"])
