@@ -32,6 +32,9 @@ int ltx_test_attention_force_split(int parts);
  * (sample, head, 256-query) units over Tk keys on `sms` SMs, the units that run whole
  * (*n_full) and the parts each remaining unit is split into (*split_k; 1: no split). */
 int ltx_test_attention_plan(int64_t units, int64_t Tk, int sms, int* n_full, int* split_k);
+/* Force CTA pairs (1) or single-CTA tiles (0) for the calling thread's subsequent
+ * ltx_linear_fp8 calls, or -1 for the automatic choice. */
+int ltx_test_fp8_force_pair(int pair);
 int ltx_test_bounded_wait(unsigned long long limit_cycles, int* returned, void* stream);
 
 #ifdef __cplusplus

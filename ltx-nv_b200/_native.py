@@ -155,6 +155,7 @@ _SIGNATURES = {
     "ltx_linear": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64,
                                   ctypes.POINTER(Epilogue), ctypes.c_int, c_vp]),
     "ltx_gemm_set_tile_n": (ctypes.c_int, [ctypes.c_int]),
+    "ltx_test_fp8_force_pair": (ctypes.c_int, [ctypes.c_int]),
     "ltx_test_bounded_wait": (ctypes.c_int, [ctypes.c_ulonglong, c_vp, c_vp]),
     "ltx_test_attention_force_split": (ctypes.c_int, [ctypes.c_int]),
     "ltx_test_attention_plan": (ctypes.c_int, [c_i64, c_i64, ctypes.c_int, ctypes.POINTER(ctypes.c_int),
@@ -673,6 +674,11 @@ def linear_fp8(a: Fp8Rows, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = N
             w.data.stride(0), w.scales.data_ptr(), c.data_ptr(), ld, a.rows, w.rows, a.cols,
             ctypes.byref(epi) if epi is not None else None, dt,
             label=f"linear_fp8 M={a.rows} N={w.rows} K={a.cols}" if _profile is not None else None)
+
+
+def fp8_force_pair(pair: int) -> None:
+    """Test hook (include/ltxb200_testing.h): force the calling thread's linear_fp8 kernel."""
+    _call("ltx_test_fp8_force_pair", pair)
 
 
 MASK_KINDS = {torch.bool: 0, torch.float32: 1, torch.bfloat16: 2}

@@ -4,6 +4,8 @@
 //   ltx_linear_fp8          C = epilogue(A W^T), A and W 8-bit rows
 // None has a counterpart in the reference, which runs its linear layers in bf16
 // (ltx_nn.py:126-158, 188-192, 244-245).
+#include <algorithm>
+
 #include "fp8.cuh"
 
 namespace ltx {
@@ -179,61 +181,105 @@ LTX_DEVICE float gelu_sigmoid(float v) {
   return __fdividef(v, 1.f + __expf(-z2));
 }
 
-// Epilogue of eight accumulators (columns [col, col + 8) of row `row`, sample sb, token st)
-// in fp32, rounded once on the store: acc + bias, then the activation, residual + gate *
-// (acc + bias), or + row_vec on marked rows. `vec`: 16-byte accesses are allowed.
-template <typename T>
-LTX_DEVICE void fp8_epilogue8(const Epi<T>& e, bool vec, T* __restrict__ crow, int64_t row, int64_t sb, int64_t st,
-                              int col, int N, float (&v)[8]) {
-  const bool whole = vec && col + 8 <= N;
-  auto load = [&](const T* p, float (&x)[8]) {
-    if (whole) {
-      ld8<T>(p, x);
-    } else {
+// 16 consecutive values, 32 (bf16) or 64 (fp32) bytes, 32-byte aligned.
+template <typename T> LTX_DEVICE void ld16v(const T* p, float (&v)[16]);
+template <> LTX_DEVICE void ld16v<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[16]) {
+  uint32_t r[8];
+  ldg_32b(p, r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = col + i < N ? ld_elem<T>(p + i) : 0.f;
-    }
+  for (int i = 0; i < 8; ++i) unpack_bf16x2(r[i], v[2 * i], v[2 * i + 1]);
+}
+template <> LTX_DEVICE void ld16v<float>(const float* p, float (&v)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r[8];
+    ldg_32b(p + 8 * h, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(r[i]);
+  }
+}
+template <typename T> LTX_DEVICE void st16v(T* p, const float (&v)[16]);
+template <> LTX_DEVICE void st16v<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[16]) {
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  stg_32b(p, r);
+}
+template <> LTX_DEVICE void st16v<float>(float* p, const float (&v)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[8 * h + i]);
+    stg_32b(p + 8 * h, r);
+  }
+}
+
+// Epilogue of W (1 or 16) accumulators, columns [col, col + W) of row `row` (sample sb, token
+// st), in fp32 and rounded once on the store: acc + bias, then the activation, residual +
+// gate * (acc + bias), or + row_vec on marked rows. W = 16 needs every vector 32-byte
+// aligned there.
+template <typename T, int W>
+LTX_DEVICE void fp8_epilogue(const Epi<T>& e, T* __restrict__ crow, int64_t row, int64_t sb, int64_t st, int col,
+                             float (&v)[W]) {
+  auto load = [](const T* p, float (&x)[W]) {
+    if constexpr (W == 16)
+      ld16v<T>(p, x);
+    else
+      x[0] = ld_elem<T>(p);
   };
-  float a[8];
+  float a[W];
   if (e.bias) {
     load(e.bias + col, a);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += a[i];
+    for (int i = 0; i < W; ++i) v[i] += a[i];
   }
   if (e.kind == LTX_EPI_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = gelu_sigmoid(v[i]);
+    for (int i = 0; i < W; ++i) v[i] = gelu_sigmoid(v[i]);
   } else if (e.kind == LTX_EPI_SILU) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fdividef(v[i], 1.f + __expf(-v[i]));
+    for (int i = 0; i < W; ++i) v[i] = __fdividef(v[i], 1.f + __expf(-v[i]));
   } else if (e.kind == LTX_EPI_GATE_RESIDUAL) {
-    float g[8];
+    float g[W];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = e.gate.on ? 0.f : 1.f;
+    for (int i = 0; i < W; ++i) g[i] = e.gate.on ? 0.f : 1.f;
     if (e.gate.table) {
       load(e.gate.table + e.gate.toff + col, a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] += a[i];
+      for (int i = 0; i < W; ++i) g[i] += a[i];
     }
     if (e.gate.mod) {
       load(e.gate.mod + sb * e.gate.ldb + st * e.gate.ldt + e.gate.moff + col, a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] += a[i];
+      for (int i = 0; i < W; ++i) g[i] += a[i];
     }
     load(e.residual + row * e.ld_res + col, a);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fmaf(g[i], v[i], a[i]);
+    for (int i = 0; i < W; ++i) v[i] = fmaf(g[i], v[i], a[i]);
   } else if (e.kind == LTX_EPI_ROW_MASK_ADD && e.row_mask[row] > 0.f) {
     load(e.row_vec + col, a);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += a[i];
+    for (int i = 0; i < W; ++i) v[i] += a[i];
   }
-  if (whole) {
-    st8<T>(crow + col, v);
+  if constexpr (W == 16)
+    st16v<T>(crow + col, v);
+  else
+    st_elem<T>(crow + col, v[0]);
+}
+// 16 columns of which those below N exist; `vec`: 32-byte accesses are allowed.
+template <typename T>
+LTX_DEVICE void fp8_epilogue_cols(const Epi<T>& e, bool vec, T* __restrict__ crow, int64_t row, int64_t sb, int64_t st,
+                                  int col, int N, float (&v)[16]) {
+  if (vec && col + 16 <= N) {
+    fp8_epilogue<T, 16>(e, crow, row, sb, st, col, v);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < N) st_elem<T>(crow + col + i, v[i]);
+    for (int i = 0; i < 16; ++i)
+      if (col + i < N) {
+        float x[1] = {v[i]};
+        fp8_epilogue<T, 1>(e, crow, row, sb, st, col + i, x);
+      }
   }
 }
 
@@ -244,24 +290,30 @@ LTX_DEVICE void fp8_epilogue8(const Epi<T>& e, bool vec, T* __restrict__ crow, i
 // takes e4m3 operands and a power of two per row and 32 values of K, so a block of 128
 // columns is one 128-byte slab of both operands and four MMAs (K = 32) that read the same
 // scale byte; sums stay in fp32 in tensor memory, no scaling is left for the CUDA cores.
-// A scale word holds four blocks, so scales move once per four slabs: 512 bytes per 128
-// rows by TMA next to the slab, then one tcgen05.cp into tensor memory, ordered with the
-// MMAs that follow it; two scale buffers alternate.
+//
+// A scale word holds four blocks, so scales move once per four slabs: 512 bytes per 128 rows
+// by TMA beside the slab (that order is the format's, fp8.cuh), then one tcgen05.cp per 128
+// rows into tensor memory, in order with the MMAs that follow it; two buffers alternate.
+// Four more warps that stored the words with tcgen05.st, off the issuing thread, were
+// slower: 660 against 565 clocks per slab at 12288 x 2048 x 8192 (the issuer waits for them).
 // ---------------------------------------------------------------------------------
 
 // One 128 x 128 tile per CTA, K split over the CTAs of a cluster (SPLIT = cluster size),
 // whose fp32 partial tiles are added through distributed shared memory in rank order:
 // short and wide problems spread over the SMs without a workspace or a second launch,
-// and the sum's order does not depend on timing.
+// and the sum's order does not depend on timing. Tiles whose output cannot be stored 32
+// bytes at a time take the same way through shared memory, so that neighbouring threads
+// store neighbouring columns.
 struct Fp8TileCfg {
   static constexpr int STAGES = 6;
   static constexpr int SLAB = 128 * 128;             // 128 rows x 128 bytes
-  static constexpr int SF = 512;                     // scale words of 128 rows, one quad
-  static constexpr int STAGE_BYTES = 2 * SLAB + 2 * SF;
+  static constexpr int SF = 512;                     // scale words of 128 rows, four slabs
+  static constexpr int STAGE_BYTES = 2 * SLAB;
+  static constexpr int RING = STAGES * STAGE_BYTES;
   static constexpr int TMEM_COLS = 256;              // accumulator [0, 128), scales [128, 144)
   static constexpr int LD_PART = 128 + 4;            // floats per row of a partial tile (no bank conflicts)
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 256 + 1024;
-  static_assert(128 * LD_PART * 4 <= STAGES * STAGE_BYTES, "the partial tile reuses the operand ring");
+  static constexpr int SMEM = RING + STAGES * 2 * SF + 256 + 1024;
+  static_assert(128 * LD_PART * 4 <= RING, "the partial tile reuses the operand ring");
 };
 
 template <typename T>
@@ -272,7 +324,8 @@ __global__ void __launch_bounds__(192, 1)
   using Cfg = Fp8TileCfg;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES);
+  uint8_t* sf_smem = smem + Cfg::RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + Cfg::STAGES * 2 * Cfg::SF);
   uint64_t* empty = full + Cfg::STAGES;
   uint64_t* tfull = empty + Cfg::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
@@ -309,6 +362,7 @@ __global__ void __launch_bounds__(192, 1)
   pdl_wait();
   pdl_trigger();
 
+  const bool staged = split > 1 || !vec;
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
@@ -316,100 +370,343 @@ __global__ void __launch_bounds__(192, 1)
         const int it = kb - kb0, s = it % Cfg::STAGES;
         if (!mbar_wait(&empty[s], (uint32_t(it / Cfg::STAGES) & 1) ^ 1, abort_flag)) break;
         uint8_t* st = smem + s * Cfg::STAGE_BYTES;
-        const bool sf = kb == kb0 || (kb & 3) == 0;  // a new scale word
-        mbar_arrive_expect_tx(&full[s], sf ? Cfg::STAGE_BYTES : 2 * Cfg::SLAB);
+        const bool quad = kb == kb0 || (kb & 3) == 0;  // a new scale word
+        mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES + (quad ? 2 * Cfg::SF : 0));
         tma_load_2d(st, &tmA, &full[s], kb * 128, m0);
         tma_load_2d(st + Cfg::SLAB, &tmB, &full[s], kb * 128, n0);
-        if (sf) {
-          tma_load_2d(st + 2 * Cfg::SLAB, &tmSA, &full[s], m0, kb >> 2);
-          tma_load_2d(st + 2 * Cfg::SLAB + Cfg::SF, &tmSB, &full[s], n0, kb >> 2);
+        if (quad) {
+          tma_load_2d(sf_smem + s * 2 * Cfg::SF, &tmSA, &full[s], m0, kb >> 2);
+          tma_load_2d(sf_smem + s * 2 * Cfg::SF + Cfg::SF, &tmSB, &full[s], n0, kb >> 2);
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int it = kb - kb0, s = it % Cfg::STAGES;
-        if (!mbar_wait(&full[s], uint32_t(it / Cfg::STAGES) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t a = smem_u32(smem + s * Cfg::STAGE_BYTES), b = a + Cfg::SLAB;
-        const uint32_t sfa = tmem + 128u + uint32_t((kb >> 2) & 1) * 8u, sfb = sfa + 4u;
-        if (kb == kb0 || (kb & 3) == 0) {
-          tmem_cp_scales(sfa, umma_desc_rows16(a + 2 * Cfg::SLAB));
-          tmem_cp_scales(sfb, umma_desc_rows16(a + 2 * Cfg::SLAB + Cfg::SF));
-        }
-        const uint32_t idesc = umma_idesc_mx8(128, 128, kb & 3);
+      const uint32_t lo0 = umma_desc_sw128_lo(smem_u32(smem)), sf0 = umma_desc_rows16_lo(smem_u32(sf_smem));
+      int s = 0;
+      uint32_t par = 0, accumulate = 0;
+      for (int kb = kb0 & ~3; ok && kb < kb1; kb += 4) {  // by scale words
+        const uint32_t sfa = tmem + 128u + uint32_t((kb >> 2) & 1) * 8u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_mx8_ss(tmem, umma_desc_sw128(a + k * 32, 16, 1024), umma_desc_sw128(b + k * 32, 16, 1024), idesc, sfa,
-                      sfb, (it > 0 || k > 0) ? 1u : 0u);
-        umma_commit(&empty[s]);
+        for (int j = 0; j < 4; ++j) {
+          if (kb + j >= kb0 && kb + j < kb1) {
+            ok = ok && mbar_wait(&full[s], par, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            if (j == 0 || kb + j == kb0) {
+              const uint32_t sf = sf0 + uint32_t(s) * (2 * Cfg::SF / 16);
+              tmem_cp_scales(sfa, umma_desc_rows16_of(sf));
+              tmem_cp_scales(sfa + 4u, umma_desc_rows16_of(sf + Cfg::SF / 16));
+            }
+            const uint32_t lo = lo0 + uint32_t(s) * (Cfg::STAGE_BYTES / 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              umma_mx8_ss(tmem, umma_desc_sw128_of(lo + 2 * k), umma_desc_sw128_of(lo + Cfg::SLAB / 16 + 2 * k),
+                          umma_idesc_mx8(128, 128, j), sfa, sfa + 4u, accumulate);
+              accumulate = 1;
+            }
+            umma_commit(&empty[s]);
+            if (++s == Cfg::STAGES) {
+              s = 0;
+              par ^= 1;
+            }
+          }
+        }
       }
       if (ok) umma_commit(tfull);
     }
   } else {
     const int q = warp & 3;  // TMEM lane quadrant
+    const uint32_t tquad = tmem + (uint32_t(q * 32) << 16);
     const int64_t m = int64_t(m0) + q * 32 + lane;
     const bool live = m < M;
-    ok = mbar_wait(tfull, 0, abort_flag);
-    if (ok) {
+    if (mbar_wait(tfull, 0, abort_flag)) {
       tc_fence_after();
-      const uint32_t tbase = tmem + (uint32_t(q * 32) << 16);
       float* part = reinterpret_cast<float*>(smem) + (q * 32 + lane) * Cfg::LD_PART;
-      const int64_t sb = m / epi.rows_per_batch, st = m - sb * epi.rows_per_batch;
+      const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
 #pragma unroll 1
       for (int c0 = 0; c0 < 128 && n0 + c0 < N; c0 += 32) {
         uint32_t rr[32];
-        tmem_ld32(tbase + uint32_t(c0), rr);
+        tmem_ld32(tquad + uint32_t(c0), rr);
         tmem_wait_ld();
         if (!live) continue;
+        if (staged) {
+          // every MMA of this CTA has read its operands: the ring is free
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (split > 1) {
-            // every MMA of this CTA has read its operands: the ring is free
-            *reinterpret_cast<uint4*>(part + c0 + 8 * j) = make_uint4(rr[8 * j], rr[8 * j + 1], rr[8 * j + 2], rr[8 * j + 3]);
-            *reinterpret_cast<uint4*>(part + c0 + 8 * j + 4) =
-                make_uint4(rr[8 * j + 4], rr[8 * j + 5], rr[8 * j + 6], rr[8 * j + 7]);
-          } else if (n0 + c0 + 8 * j < N) {
-            float v[8];
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(part + c0 + j) = make_uint4(rr[j], rr[j + 1], rr[j + 2], rr[j + 3]);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(rr[8 * j + e]);
-            fp8_epilogue8<T>(epi, vec, C + m * ldc, m, sb, st, n0 + c0 + 8 * j, N, v);
+          for (int j = 0; j < 32; j += 16) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(rr[j + e]);
+            fp8_epilogue_cols<T>(epi, true, C + m * ldc, m, sb, st, n0 + c0 + j, N, v);
           }
         }
       }
     }
   }
   __syncwarp();
-  if (split > 1) {
-    cluster_sync_all();
-    // CTA `rank` finishes the tile's column groups of 8 with index % split == rank
-    const int rows = min(128, M - m0), groups = (min(128, N - n0) + 7) / 8;
-    const int mine = (groups - rank + split - 1) / split;
-    const uint32_t base = smem_u32(smem);
-    for (int i = threadIdx.x; i < rows * mine; i += blockDim.x) {
-      const int r = i / mine, c = ((i - r * mine) * split + rank) * 8;
-      float v[8] = {};
-      for (int p = 0; p < split; ++p) {
-        const uint32_t at = mapa_shared(base, uint32_t(p)) + uint32_t(r * Cfg::LD_PART + c) * 4u;
-        const float4 x = ld_cluster_f4(at), y = ld_cluster_f4(at + 16);
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+  if (staged) {
+    if (split > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    const int rows = min(128, M - m0), cols = min(128, N - n0);
+    uint32_t base[8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) base[p] = p < split ? mapa_shared(smem_u32(smem), uint32_t(p)) : 0u;
+    if (vec) {
+      // CTA `rank` finishes the tile's groups of 16 columns with index % split == rank
+      const int groups = (cols + 15) / 16, mine = (groups - rank + split - 1) / split;
+      for (int i = threadIdx.x; i < rows * mine; i += 192) {
+        const int r = i / mine, c = ((i - r * mine) * split + rank) * 16;
+        float v[16] = {};
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          if (p < split) {
+            const uint32_t at = base[p] + uint32_t(r * Cfg::LD_PART + c) * 4u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 x = ld_cluster_f4(at + 16 * j);
+              v[4 * j] += x.x;
+              v[4 * j + 1] += x.y;
+              v[4 * j + 2] += x.z;
+              v[4 * j + 3] += x.w;
+            }
+          }
+        }
+        const int64_t m = int64_t(m0) + r;
+        const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
+        fp8_epilogue_cols<T>(epi, true, C + m * ldc, m, sb, st, n0 + c, N, v);
       }
-      const int64_t m = int64_t(m0) + r;
-      const int64_t sb = m / epi.rows_per_batch, st = m - sb * epi.rows_per_batch;
-      fp8_epilogue8<T>(epi, vec, C + m * ldc, m, sb, st, n0 + c, N, v);
+    } else {
+      // one element per thread, the ranks taking the rows in turn
+      for (int i = threadIdx.x; i < (rows - rank + split - 1) / split * 128; i += 192) {
+        const int r = (i >> 7) * split + rank, c = i & 127;
+        if (c >= cols) continue;
+        float v[1] = {0.f};
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p < split) v[0] += ld_cluster_f1(base[p] + uint32_t(r * Cfg::LD_PART + c) * 4u);
+        const int64_t m = int64_t(m0) + r;
+        const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
+        fp8_epilogue<T, 1>(epi, C + m * ldc, m, sb, st, n0 + c, v);
+      }
     }
-    cluster_sync_all();  // no CTA leaves while another reads its partial tile
+    if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its partial tile
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// Large problems: a CTA pair (cluster of two SMs, cta_group::2 MMAs) per 256 x 256 tile,
+// persistent over the tiles, N fastest so that the rows of A stay in L2. Each CTA loads its
+// 128 rows of A and 128 of the 256 rows of W (32 KB per slab and SM for 512 clocks of MMA);
+// its tensor memory holds its rows' scales and those of all 256 columns.
+//
+// Two 256-column accumulators and two scale buffers of 12 columns do not fit in 512, so the
+// accumulators share 32 columns, [224, 256): the epilogue of a tile reads that slab first
+// and lets the next tile's MMAs start behind it (`tover`), long before the whole
+// accumulator is drained (`tempty`, which the tile after next waits for). Those arrivals
+// cross to the leader without a release: they order tensor-memory reads, which
+// tcgen05.wait and the fence have completed, and no other memory; with a cluster-scope
+// release each cost 1.2 us behind the tile's stores (725 -> 635 clocks per slab at
+// 12288 x 8192 x 2048).
+struct Fp8PairCfg {
+  static constexpr int STAGES = 6;
+  static constexpr int SLAB = 128 * 128;
+  static constexpr int SF_A = 512, SF_B = 1024;  // scale words of 128 / 256 rows, four slabs
+  static constexpr int SF = SF_A + SF_B;
+  static constexpr int RING = STAGES * 2 * SLAB;
+  static constexpr int SMEM = RING + STAGES * SF + 256 + 1024;
+  static constexpr uint32_t ACC1 = 224;    // accumulator 1 at [224, 480), accumulator 0 at [0, 256)
+  static constexpr uint32_t SF_COL = 480;  // two buffers of 4 (A) + 8 (W) columns
+};
+
+// Warp 0 TMA, warp 1 MMA issuer (leader), warps 2-9 epilogue.
+template <typename T>
+__global__ void __launch_bounds__(320, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                         T* __restrict__ C, int64_t ldc, int M, int N, int K, int vec, Epi<T> epi) {
+  using Cfg = Fp8PairCfg;
+  constexpr int S = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint8_t* sf_smem = smem + Cfg::RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sf_smem + S * Cfg::SF);
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* tover = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tover + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  const int warp = warp_id(), lane = lane_id();
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int n_tiles = (N + 255) / 256, num_tiles = ((M + 255) / 256) * n_tiles;
+  const int k_blocks = (K + 127) / 128;
+  const int tile0 = int(blockIdx.x >> 1), tile_step = int(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 16);  // every epilogue warp of both CTAs
+    }
+    mbar_init(tover, 8);  // the four warps of both CTAs that read the shared slab
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmSB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();  // both CTAs' barriers and tensor memory before any cross-CTA use
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < num_tiles; tile += tile_step) {
+        const int m0 = (tile / n_tiles) * 256 + int(rank) * 128, n0 = (tile % n_tiles) * 256;
+        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+          const int s = it % S;
+          ok = mbar_wait(&empty[s], (uint32_t(it / S) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          uint8_t* sa = smem + s * 2 * Cfg::SLAB;
+          const uint32_t fb = mapa_shared(smem_u32(&full[s]), 0);  // both CTAs' bytes complete on the leader's
+          const bool quad = (kb & 3) == 0;                             // a new scale word
+          if (leader) mbar_arrive_expect_tx(&full[s], 4 * Cfg::SLAB + (quad ? 2 * Cfg::SF : 0));
+          tma_load_2d_pair(sa, &tmA, fb, kb * 128, m0);
+          tma_load_2d_pair(sa + Cfg::SLAB, &tmB, fb, kb * 128, n0 + int(rank) * 128);
+          if (quad) {
+            tma_load_2d_pair(sf_smem + s * Cfg::SF, &tmSA, fb, m0, kb >> 2);
+            tma_load_2d_pair(sf_smem + s * Cfg::SF + Cfg::SF_A, &tmSB, fb, n0, kb >> 2);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // One thread issues every MMA, so its own instructions count: the descriptors' constant
+    // halves are built once and stages and parities are kept, not divided out (0.185 ms ->
+    // 0.15 ms at 12288 x 8192 x 2048, 986 -> 785 clocks per slab).
+    if (lane == 0 && leader) {
+      const uint32_t lo0 = umma_desc_sw128_lo(smem_u32(smem)), sf0 = umma_desc_rows16_lo(smem_u32(sf_smem));
+      int s = 0, local = 0;
+      uint32_t par = 0, sfa = tmem + Cfg::SF_COL;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < num_tiles; tile += tile_step, ++local) {
+        const int acc = local & 1;
+        ok = mbar_wait(&tempty[acc], (uint32_t(local >> 1) & 1) ^ 1, abort_flag) &&
+             (local == 0 || mbar_wait(tover, uint32_t(local - 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (acc ? Cfg::ACC1 : 0u);
+        uint32_t accumulate = 0;
+        for (int kb = 0; kb < k_blocks; kb += 4) {
+          const int n = min(4, k_blocks - kb);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j < n) {
+              ok = ok && mbar_wait(&full[s], par, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              if (j == 0) {
+                const uint32_t sf = sf0 + uint32_t(s) * (Cfg::SF / 16);
+                tmem_cp_scales_pair(sfa, umma_desc_rows16_of(sf));
+                tmem_cp_scales_pair(sfa + 4u, umma_desc_rows16_of(sf + Cfg::SF_A / 16));
+                tmem_cp_scales_pair(sfa + 8u, umma_desc_rows16_of(sf + Cfg::SF_A / 16 + 32));
+              }
+              const uint32_t lo = lo0 + uint32_t(s) * (2 * Cfg::SLAB / 16);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                umma_mx8_ss_pair(d, umma_desc_sw128_of(lo + 2 * k), umma_desc_sw128_of(lo + Cfg::SLAB / 16 + 2 * k),
+                                 umma_idesc_mx8(256, 256, j), sfa, sfa + 4u, accumulate);
+                accumulate = 1;
+              }
+              umma_commit_pair(&empty[s], 3);
+              if (++s == S) {
+                s = 0;
+                par ^= 1;
+              }
+            }
+          }
+          if (!ok) break;
+          sfa = 2 * (tmem + Cfg::SF_COL) + 12u - sfa;  // the other buffer
+        }
+        if (ok) umma_commit_pair(&tfull[acc], 3);
+      }
+    }
+  } else {
+    // Epilogue warps 2..9: TMEM lane quadrant warp % 4 (one accumulator row per thread),
+    // column half (warp - 2) / 4.
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    int local = 0;
+    for (int tile = tile0; tile < num_tiles; tile += tile_step, ++local) {
+      const int acc = local & 1;
+      const int m0 = (tile / n_tiles) * 256 + int(rank) * 128, n0 = (tile % n_tiles) * 256;
+      const int64_t m = int64_t(m0) + q * 32 + lane;
+      const bool live = m < M;
+      const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
+      if (!mbar_wait(&tfull[acc], uint32_t(local >> 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t tbase = tmem + (acc ? Cfg::ACC1 : 0u) + (uint32_t(q * 32) << 16);
+      // accumulator 0 shares its last slab (half 1), accumulator 1 its first (half 0)
+      const bool shares = half == (acc ^ 1);
+      T* crow = C + m * ldc;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        const int c0 = half * 128 + (acc ? j : 3 - j) * 32;
+        uint32_t rr[32];
+        tmem_ld32(tbase + uint32_t(c0), rr);
+        tmem_wait_ld();
+        if (j == 0 && shares) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(tover), 0));
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int c = 0; c < 32; c += 16) {
+          if (n0 + c0 + c < N) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(rr[c + e]);
+            fp8_epilogue_cols<T>(epi, vec, crow, m, sb, st, n0 + c0 + c, N, v);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&tempty[acc]), 0));
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // no CTA of the pair leaves while the other may still signal its barriers
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -422,22 +719,42 @@ inline int fp8_split(int64_t tiles, int64_t k_blocks) {
 }
 
 template <typename T>
-void launch_fp8_tile(const void* A, int64_t lda, const void* As, const void* W, int64_t ldw, const void* Ws, T* C,
-                     int64_t ldc, int64_t M, int64_t N, int64_t K, const Epi<T>& epi, bool vec, cudaStream_t s) {
-  using Cfg = Fp8TileCfg;
-  const uint64_t quads = uint64_t(fp8_quads(K));
+void launch_linear_fp8(const void* A, int64_t lda, const void* As, const void* W, int64_t ldw, const void* Ws, T* C,
+                       int64_t ldc, int64_t M, int64_t N, int64_t K, const Epi<T>& epi, bool vec, bool pair,
+                       cudaStream_t s) {
   const CUtensorMap ta = make_tmap_u8_2d(A, uint64_t(K), uint64_t(M), uint64_t(lda), 128);
   const CUtensorMap tb = make_tmap_u8_2d(W, uint64_t(K), uint64_t(N), uint64_t(ldw), 128);
+  const uint64_t quads = uint64_t(fp8_quads(K));
   const CUtensorMap tsa = make_tmap_u32_2d(As, uint64_t(fp8_rows_padded(M)), quads, 128);
-  const CUtensorMap tsb = make_tmap_u32_2d(Ws, uint64_t(fp8_rows_padded(N)), quads, 128);
+  const CUtensorMap tsb = make_tmap_u32_2d(Ws, uint64_t(fp8_rows_padded(N)), quads, pair ? 256 : 128);
+  static std::atomic<uint64_t> smem_done[2] = {};
+  if (pair) {
+    auto kern = gemm_fp8_pair_kernel<T>;
+    ensure_smem_limit(smem_done[1], kern, Fp8PairCfg::SMEM);
+    const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
+    LTX_UNSUPPORTED(tiles < (int64_t(1) << 31) - 65536, "too many tiles for one launch");
+    const int64_t pairs = std::min<int64_t>(num_sms() / 2, tiles);
+    launch_pdl(kern, dim3(unsigned(2 * pairs)), dim3(320), Fp8PairCfg::SMEM, s, 2, ta, tb, tsa, tsb, C, ldc, int(M),
+               int(N), int(K), int(vec), epi);
+    return;
+  }
   auto kern = gemm_fp8_tile_kernel<T>;
-  static std::atomic<uint64_t> smem_done{0};
-  ensure_smem_limit(smem_done, kern, Cfg::SMEM);
+  ensure_smem_limit(smem_done[0], kern, Fp8TileCfg::SMEM);
   const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
   const int split = fp8_split(tiles, (K + 127) / 128);
   LTX_UNSUPPORTED(tiles * split < (int64_t(1) << 31), "too many tiles for one launch");
-  launch_pdl(kern, dim3(unsigned(tiles * split)), dim3(192), Cfg::SMEM, s, unsigned(split), ta, tb, tsa, tsb, C, ldc,
-             int(M), int(N), int(K), split, int(vec), epi);
+  launch_pdl(kern, dim3(unsigned(tiles * split)), dim3(192), Fp8TileCfg::SMEM, s, unsigned(split), ta, tb, tsa, tsb, C,
+             ldc, int(M), int(N), int(K), split, int(vec), epi);
+}
+
+// Test hook (ltx_test_fp8_force_pair): -1 automatic, 0 single-CTA tiles, 1 CTA pairs.
+static thread_local int g_fp8_force_pair = -1;
+
+// CTA pairs from the size on at which their tiles keep most SMs busy (outputs that cannot
+// be stored 32 bytes at a time go through the tile kernel's staging).
+inline bool fp8_use_pair(int64_t M, int64_t N, bool vec) {
+  if (g_fp8_force_pair >= 0) return g_fp8_force_pair != 0;
+  return vec && ((M + 255) / 256) * ((N + 255) / 256) * 2 >= num_sms() / 2;
 }
 
 }  // namespace detail
@@ -450,7 +767,7 @@ namespace {
 
 // ltx_epilogue as the 8-bit products take it: the same fields as make_epi, but vectors of
 // any alignment and stride (a column count that is not a multiple of 8 has them).
-// `vec` tells whether every vector may be read 16 bytes at a time.
+// `vec` tells whether every vector may be read 32 bytes at a time.
 template <typename T>
 Epi<T> make_epi_any(const ltx_epilogue* p, int64_t N, bool& vec) {
   Epi<T> e;
@@ -459,7 +776,7 @@ Epi<T> make_epi_any(const ltx_epilogue* p, int64_t N, bool& vec) {
   auto take = [&](const void* ptr) {
     if (reinterpret_cast<uintptr_t>(ptr) % sizeof(T))
       throw ApiError{LTX_ERR_INVALID, "an epilogue vector is not aligned to its type"};
-    if (reinterpret_cast<uintptr_t>(ptr) % 16) vec = false;
+    if (reinterpret_cast<uintptr_t>(ptr) % 32) vec = false;
     return static_cast<const T*>(ptr);
   };
   if (p->kind < LTX_EPI_NONE || p->kind > LTX_EPI_ROW_MASK_ADD)
@@ -467,13 +784,14 @@ Epi<T> make_epi_any(const ltx_epilogue* p, int64_t N, bool& vec) {
   if (p->silu_input) throw ApiError{LTX_ERR_INVALID, "silu_input is not an epilogue of 8-bit rows"};
   e.kind = p->kind;
   e.bias = take(p->bias);
-  e.rows_per_batch = p->rows_per_batch > 0 ? p->rows_per_batch : 1;
+  // rows are below 2^31: a longer sample is all of them (the kernels divide in 32 bits)
+  e.rows_per_batch = p->rows_per_batch > 0 ? std::min<int64_t>(p->rows_per_batch, INT32_MAX) : 1;
   if (e.kind == LTX_EPI_GATE_RESIDUAL) {
     if (p->residual == nullptr) throw ApiError{LTX_ERR_INVALID, "GATE_RESIDUAL needs a residual"};
     if (p->ld_residual < N) throw ApiError{LTX_ERR_INVALID, "ld_residual must hold the columns"};
     e.residual = take(p->residual);
     e.ld_res = p->ld_residual;
-    if (e.ld_res % 8) vec = false;
+    if (e.ld_res % 16) vec = false;
     const ltx_modulation& g = p->gate;
     if (g.has_scale && (g.table != nullptr || g.mod != nullptr)) {
       e.gate.table = take(g.table);
@@ -483,7 +801,7 @@ Epi<T> make_epi_any(const ltx_epilogue* p, int64_t N, bool& vec) {
       e.gate.toff = g.scale_table_off;
       e.gate.moff = g.scale_mod_off;
       e.gate.on = 1;
-      if ((e.gate.ldb % 8) || (e.gate.ldt % 8) || (e.gate.toff % 8) || (e.gate.moff % 8)) vec = false;
+      if ((e.gate.ldb % 16) || (e.gate.ldt % 16) || (e.gate.toff % 16) || (e.gate.moff % 16)) vec = false;
     }
   }
   if (e.kind == LTX_EPI_ROW_MASK_ADD) {
@@ -626,13 +944,20 @@ extern "C" int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, 
     using T = std::remove_pointer_t<decltype(cp)>;
     bool vec;
     const Epi<T> e = make_epi_any<T>(epi, N, vec);
-    vec = vec && vec_ok(C, ldc);
-    launch_fp8_tile<T>(A, lda, a_scales, W, ldw, w_scales, cp, ldc, M, N, K, e, vec, s);
+    vec = vec && reinterpret_cast<uintptr_t>(C) % 32 == 0 && ldc % 16 == 0;
+    launch_linear_fp8<T>(A, lda, a_scales, W, ldw, w_scales, cp, ldc, M, N, K, e, vec, fp8_use_pair(M, N, vec), s);
   };
   if (dtype == LTX_F32)
     run(static_cast<float*>(C));
   else
     run(static_cast<__nv_bfloat16*>(C));
   LTX_CUDA(cudaGetLastError());
+  LTX_API_END
+}
+
+extern "C" int ltx_test_fp8_force_pair(int pair) {
+  LTX_API_BEGIN
+  LTX_REQUIRE(pair >= -1 && pair <= 1, "pair must be -1, 0 or 1");
+  g_fp8_force_pair = pair;
   LTX_API_END
 }

@@ -242,6 +242,12 @@ LTX_DEVICE uint32_t mapa_shared(uint32_t local_smem_addr, uint32_t rank) {
 LTX_DEVICE void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same without a release: for arrivals that order tensor-memory accesses only, which
+// tcgen05.wait / fence have completed. A release at cluster scope waits for the thread's
+// earlier global stores.
+LTX_DEVICE void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // 2D tiled TMA load into this CTA's shared memory whose completion bytes are counted on
 // the barrier at `bar_cluster_addr` (the leader CTA's barrier for a CTA pair).
 LTX_DEVICE void tma_load_2d_pair(void* dst, const void* tmap, uint32_t bar_cluster_addr, int x, int y) {
@@ -355,15 +361,31 @@ __host__ __device__ constexpr uint32_t umma_idesc_mx8(int M, int N, int sf) {
 }
 // 32 rows of 16 bytes (512 contiguous bytes of shared memory) -> 4 columns of tensor
 // memory, repeated in the four 32-lane quadrants: the scale words of 128 operand rows.
-// Ordered with the MMAs of the same thread.
-LTX_DEVICE uint64_t umma_desc_rows16(uint32_t smem_addr) {
-  return uint64_t((smem_addr & 0x3FFFF) >> 4) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+// In order with the MMAs of the same thread. The descriptor in two steps, as above.
+LTX_DEVICE uint32_t umma_desc_rows16_lo(uint32_t smem_addr) { return (smem_addr & 0x3FFFF) >> 4; }
+LTX_DEVICE uint64_t umma_desc_rows16_of(uint32_t lo) {
+  constexpr uint32_t hi = (128u >> 4) | (1u << 14);
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
 }
 LTX_DEVICE void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 LTX_DEVICE void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// 32 bytes at once (32-byte aligned): one full sector per thread.
+LTX_DEVICE void ldg_32b(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p)
+               : "memory");
+}
+LTX_DEVICE void stg_32b(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 // 4 and 16 bytes of another CTA's shared memory, by its shared::cluster address.
 LTX_DEVICE float ld_cluster_f1(uint32_t cluster_addr) {
@@ -400,6 +422,16 @@ LTX_DEVICE uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t s
   d |= uint64_t((sbo >> 4) & 0x3FFF) << 32;
   d |= uint64_t(1) << 46;  // descriptor version for sm_100
   d |= uint64_t(2) << 61;  // SWIZZLE_128B
+  return d;
+}
+
+// The same descriptor for K-major operands (lbo 16, sbo 1024) in two steps: its low word
+// for an address, to which 16-byte steps may be added, and the whole from the low word.
+LTX_DEVICE uint32_t umma_desc_sw128_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFF) >> 4) | (1u << 16); }
+LTX_DEVICE uint64_t umma_desc_sw128_of(uint32_t lo) {
+  constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
   return d;
 }
 

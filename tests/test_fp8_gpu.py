@@ -194,11 +194,19 @@ def check(got, want, slack, dtype):
 
 SHAPES = [(1, 1, 1), (1, 8, 16), (2, 12288, 2048), (3, 5, 100), (31, 256, 128), (32, 128, 129), (33, 300, 512),
           (100, 72, 4096), (127, 129, 130), (128, 128, 1024), (129, 257, 640), (252, 6176, 2048), (256, 512, 513),
-          (257, 1371, 1037), (300, 2048, 8192), (1000, 96, 64), (1025, 776, 1536), (2048, 2304, 256)]
+          (257, 1371, 1037), (300, 2048, 8192), (1000, 96, 64), (1025, 776, 1536), (2048, 2304, 256),
+          (3000, 4100, 384), (2560, 5120, 1040)]  # more than one tile per SM pair
+
+
+@pytest.fixture(params=[-1, 0, 1], ids=["auto", "tile", "pair"])
+def kernel(request):
+    nat.fp8_force_pair(request.param)
+    yield request.param
+    nat.fp8_force_pair(-1)
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_linear_fp8_bf16(m, n, k):
+def test_linear_fp8_bf16(m, n, k, kernel):
     """The operands are exact in float64, so only the sums' and the result's rounding is
     allowed: a sum of k terms in fp32 is off by at most k 2^-23 of sum|a w| whatever the
     order and whether an addition rounds or truncates."""
@@ -218,7 +226,7 @@ def test_linear_fp8_bf16(m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(1, 40, 300), (2, 2048, 1024), (70, 100, 520), (300, 515, 1037), (512, 768, 256)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_linear_fp8_epilogues(m, n, k, dtype):
+def test_linear_fp8_epilogues(m, n, k, dtype, kernel):
     """Every epilogue, in both result types; the activations' own arithmetic (an exponential
     of 2 units, a quotient of 2) adds 8 * 2^-23 of the value."""
     g, x, w = linear_case(m * 3 + n, m, n, k, dtype)
@@ -251,7 +259,7 @@ def test_linear_fp8_epilogues(m, n, k, dtype):
     check(out, lin + mask.double().cpu()[:, None] * vec.double().cpu(), slack + lin.abs() * 2.0 ** -23, dtype)
 
 
-def test_linear_fp8_gate_per_sample_and_per_token():
+def test_linear_fp8_gate_per_sample_and_per_token(kernel):
     g = gen(17)
     b, t, k, n = 3, 150, 256, 320
     x, w, res = randn(g, b, t, k), nat.quantize_fp8(randn(g, n, k, std=0.06)), randn(g, b, t, n)
@@ -263,7 +271,7 @@ def test_linear_fp8_gate_per_sample_and_per_token():
                                                                   gate=gate[i:i + 1]))
 
 
-def test_linear_fp8_writes_its_rows_and_columns_only():
+def test_linear_fp8_writes_its_rows_and_columns_only(kernel):
     g = gen(18)
     for m, n, k in ((5, 100, 64), (130, 264, 200), (300, 300, 512)):
         x, w = nat.quantize_fp8(randn(g, m, k)), nat.quantize_fp8(randn(g, n, k))
@@ -276,7 +284,7 @@ def test_linear_fp8_writes_its_rows_and_columns_only():
             assert torch.equal(dense, buf[:m, :n])
 
 
-def test_linear_fp8_nan_rows_stay_in_their_rows():
+def test_linear_fp8_nan_rows_stay_in_their_rows(kernel):
     """NaN and infinite activations make their own rows NaN, a NaN weight its column; what
     lies behind the last row or column of an operand reaches nothing."""
     g = gen(19)
@@ -292,7 +300,7 @@ def test_linear_fp8_nan_rows_stay_in_their_rows():
     assert torch.equal(got[~bad], clean[~bad])
 
 
-def test_linear_fp8_wide_range_of_scales():
+def test_linear_fp8_wide_range_of_scales(kernel):
     """Blocks whose scales differ by 2^60 within a row: each product is scaled exactly."""
     g = gen(20)
     k = 128 * 9
