@@ -5,6 +5,7 @@
 // None has a counterpart in the reference, which runs its linear layers in bf16
 // (ltx_nn.py:126-158, 188-192, 244-245).
 #include <algorithm>
+#include <cmath>
 
 #include "fp8.cuh"
 
@@ -181,6 +182,24 @@ LTX_DEVICE float gelu_sigmoid(float v) {
   return __fdividef(v, 1.f + __expf(-z2));
 }
 
+// 4 consecutive values, 8 (bf16) or 16 (fp32) bytes, aligned.
+template <typename T> LTX_DEVICE void ld4v(const T* p, float (&v)[4]);
+template <> LTX_DEVICE void ld4v<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  unpack_bf16x2(u.x, v[0], v[1]);
+  unpack_bf16x2(u.y, v[2], v[3]);
+}
+template <> LTX_DEVICE void ld4v<float>(const float* p, float (&v)[4]) {
+  const float4 u = *reinterpret_cast<const float4*>(p);
+  v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+}
+template <typename T> LTX_DEVICE void st4v(T* p, const float (&v)[4]);
+template <> LTX_DEVICE void st4v<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+template <> LTX_DEVICE void st4v<float>(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
 // 16 consecutive values, 32 (bf16) or 64 (fp32) bytes, 32-byte aligned.
 template <typename T> LTX_DEVICE void ld16v(const T* p, float (&v)[16]);
 template <> LTX_DEVICE void ld16v<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[16]) {
@@ -215,16 +234,17 @@ template <> LTX_DEVICE void st16v<float>(float* p, const float (&v)[16]) {
   }
 }
 
-// Epilogue of W (1 or 16) accumulators, columns [col, col + W) of row `row` (sample sb, token
+// Epilogue of W (1, 4 or 16) accumulators, columns [col, col + W) of row `row` (sample sb, token
 // st), in fp32 and rounded once on the store: acc + bias, then the activation, residual +
-// gate * (acc + bias), or + row_vec on marked rows. W = 16 needs every vector 32-byte
-// aligned there.
+// gate * (acc + bias), or + row_vec on marked rows. W > 1 needs every vector aligned there.
 template <typename T, int W>
 LTX_DEVICE void fp8_epilogue(const Epi<T>& e, T* __restrict__ crow, int64_t row, int64_t sb, int64_t st, int col,
                              float (&v)[W]) {
   auto load = [](const T* p, float (&x)[W]) {
     if constexpr (W == 16)
       ld16v<T>(p, x);
+    else if constexpr (W == 4)
+      ld4v<T>(p, x);
     else
       x[0] = ld_elem<T>(p);
   };
@@ -264,6 +284,8 @@ LTX_DEVICE void fp8_epilogue(const Epi<T>& e, T* __restrict__ crow, int64_t row,
   }
   if constexpr (W == 16)
     st16v<T>(crow + col, v);
+  else if constexpr (W == 4)
+    st4v<T>(crow + col, v);
   else
     st_elem<T>(crow + col, v[0]);
 }
@@ -298,14 +320,15 @@ LTX_DEVICE void fp8_epilogue_cols(const Epi<T>& e, bool vec, T* __restrict__ cro
 // slower: 660 against 565 clocks per slab at 12288 x 2048 x 8192 (the issuer waits for them).
 // ---------------------------------------------------------------------------------
 
-// One 128 x 128 tile per CTA, K split over the CTAs of a cluster (SPLIT = cluster size),
-// whose fp32 partial tiles are added through distributed shared memory in rank order:
-// short and wide problems spread over the SMs without a workspace or a second launch,
-// and the sum's order does not depend on timing. Tiles whose output cannot be stored 32
-// bytes at a time take the same way through shared memory, so that neighbouring threads
-// store neighbouring columns.
+// One 128 x 128 tile per CTA, K split over the `split` CTAs of a cluster, whose fp32 partial
+// tiles are added through distributed shared memory in rank order: short and wide problems
+// spread over the SMs without a workspace or a second launch, and the sum's order does not
+// depend on timing. Tiles whose output cannot be stored 32 bytes at a time take the same
+// way through shared memory, so that neighbouring threads store neighbouring columns. Two
+// CTAs with three stages each share an SM, so that one starts and ends under the other's
+// MMAs (12288 x 2048 x 2048: 61.6 us, 124 us with one CTA of six stages).
 struct Fp8TileCfg {
-  static constexpr int STAGES = 6;
+  static constexpr int STAGES = 3;
   static constexpr int SLAB = 128 * 128;             // 128 rows x 128 bytes
   static constexpr int SF = 512;                     // scale words of 128 rows, four slabs
   static constexpr int STAGE_BYTES = 2 * SLAB;
@@ -316,8 +339,60 @@ struct Fp8TileCfg {
   static_assert(128 * LD_PART * 4 <= RING, "the partial tile reuses the operand ring");
 };
 
+// Rows rank, rank + SPLIT, .. of the tile whose SPLIT fp32 partials lie at `base` in the
+// cluster's CTAs: added in rank order, epilogue, store. One warp per row, so that a part's
+// row is one contiguous 512-byte read, and 8 / SPLIT rows at a time, so that 8 reads are in
+// flight (with a lane per row the reads of 128 rows and 8 parts took 20 us).
+template <typename T, int SPLIT>
+LTX_DEVICE void fp8_add_parts(const Epi<T>& epi, bool vec, T* __restrict__ C, int64_t ldc, int m0, int n0, int rows,
+                              int cols, int rank, uint32_t base) {
+  constexpr int U = 8 / SPLIT;
+  const int lane = lane_id();
+  uint32_t part[SPLIT];
+#pragma unroll
+  for (int p = 0; p < SPLIT; ++p) part[p] = (SPLIT > 1 ? mapa_shared(base, uint32_t(p)) : base) + (vec ? 16u : 4u) * lane;
+  for (int r0 = warp_id() * SPLIT * U + rank; r0 < rows; r0 += 6 * SPLIT * U) {
+    float4 x[U][SPLIT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = min(r0 + u * SPLIT, rows - 1);
+      const uint32_t at = uint32_t(r * Fp8TileCfg::LD_PART) * 4u;
+#pragma unroll
+      for (int p = 0; p < SPLIT; ++p)
+        x[u][p] = vec ? ld_cluster_f4(part[p] + at)
+                      : make_float4(ld_cluster_f1(part[p] + at), ld_cluster_f1(part[p] + at + 128),
+                                    ld_cluster_f1(part[p] + at + 256), ld_cluster_f1(part[p] + at + 384));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * SPLIT;
+      if (r >= rows) break;
+      float v[4] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w};
+#pragma unroll
+      for (int p = 1; p < SPLIT; ++p) {
+        v[0] += x[u][p].x;
+        v[1] += x[u][p].y;
+        v[2] += x[u][p].z;
+        v[3] += x[u][p].w;
+      }
+      const int64_t m = int64_t(m0) + r;
+      const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
+      if (vec && lane * 4 + 4 <= cols) {
+        fp8_epilogue<T, 4>(epi, C + m * ldc, m, sb, st, n0 + lane * 4, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = vec ? lane * 4 + j : lane + 32 * j;
+          float w[1] = {v[j]};
+          if (c < cols) fp8_epilogue<T, 1>(epi, C + m * ldc, m, sb, st, n0 + c, w);
+        }
+      }
+    }
+  }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(192, 2)
     gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                          const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                          T* __restrict__ C, int64_t ldc, int M, int N, int K, int split, int vec, Epi<T> epi) {
@@ -454,46 +529,12 @@ __global__ void __launch_bounds__(192, 1)
     else
       __syncthreads();
     const int rows = min(128, M - m0), cols = min(128, N - n0);
-    uint32_t base[8];
-#pragma unroll
-    for (int p = 0; p < 8; ++p) base[p] = p < split ? mapa_shared(smem_u32(smem), uint32_t(p)) : 0u;
-    if (vec) {
-      // CTA `rank` finishes the tile's groups of 16 columns with index % split == rank
-      const int groups = (cols + 15) / 16, mine = (groups - rank + split - 1) / split;
-      for (int i = threadIdx.x; i < rows * mine; i += 192) {
-        const int r = i / mine, c = ((i - r * mine) * split + rank) * 16;
-        float v[16] = {};
-#pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          if (p < split) {
-            const uint32_t at = base[p] + uint32_t(r * Cfg::LD_PART + c) * 4u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float4 x = ld_cluster_f4(at + 16 * j);
-              v[4 * j] += x.x;
-              v[4 * j + 1] += x.y;
-              v[4 * j + 2] += x.z;
-              v[4 * j + 3] += x.w;
-            }
-          }
-        }
-        const int64_t m = int64_t(m0) + r;
-        const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
-        fp8_epilogue_cols<T>(epi, true, C + m * ldc, m, sb, st, n0 + c, N, v);
-      }
-    } else {
-      // one element per thread, the ranks taking the rows in turn
-      for (int i = threadIdx.x; i < (rows - rank + split - 1) / split * 128; i += 192) {
-        const int r = (i >> 7) * split + rank, c = i & 127;
-        if (c >= cols) continue;
-        float v[1] = {0.f};
-#pragma unroll
-        for (int p = 0; p < 8; ++p)
-          if (p < split) v[0] += ld_cluster_f1(base[p] + uint32_t(r * Cfg::LD_PART + c) * 4u);
-        const int64_t m = int64_t(m0) + r;
-        const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
-        fp8_epilogue<T, 1>(epi, C + m * ldc, m, sb, st, n0 + c, v);
-      }
+    const uint32_t base = smem_u32(smem);
+    switch (split) {
+      case 1: fp8_add_parts<T, 1>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
+      case 2: fp8_add_parts<T, 2>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
+      case 4: fp8_add_parts<T, 4>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
+      default: fp8_add_parts<T, 8>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
     }
     if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its partial tile
   }
@@ -710,18 +751,46 @@ __global__ void __launch_bounds__(320, 1)
   }
 }
 
-// CTAs of one cluster over K: as many as keep the grid within the SMs, at least two
-// slabs each, 1, 2, 4 or 8.
-inline int fp8_split(int64_t tiles, int64_t k_blocks) {
+// Which kernel, and over how many CTAs of a cluster the tile kernel splits K. Microseconds
+// measured on the B200 (graph replay, weights not in L2), at M x N x K:
+//   tile kernel  4.0 + 0.37 per slab of a CTA, times the CTAs per SM; adding the parts of a
+//                split costs 3.4 / 2.4 / 3.8 for 2 / 4 / 8 of them, 0.7 with few rows
+//                (126 x 2048 x 2048: 10.0 whole, 10.5 / 7.8 / 9.0 split; 2 x 1024 x 8192: 29.2
+//                whole, 16.7 / 10.2 / 7.2 split; 12288 x 2048 x 2048: 61.6)
+//   CTA pairs    4.5 + 0.5 per tile and 0.4 per slab of a pair (1024 x 4096 x 4096: 16.9
+//                against 29.6; 1024 x 1024 x 1024: 7.8 against 6.5)
+// Outputs that cannot be stored 32 bytes at a time take the tile kernel's staging.
+struct Fp8Plan {
+  bool pair = false;
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= num_sms() && k_blocks >= 4 * split) split *= 2;
-  return split;
+};
+static thread_local int g_fp8_force_pair = -1;  // ltx_test_fp8_force_pair
+
+inline Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool vec, int sms) {
+  const double kb = double((K + 127) / 128);
+  const double tiles = double((M + 127) / 128) * double((N + 127) / 128);
+  constexpr double kAdd[4] = {0.0, 3.4, 2.4, 3.8};
+  Fp8Plan p;
+  double best = 0;
+  for (int i = 0, split = 1; i < 4; ++i, split *= 2) {
+    if (split > 1 && (tiles * split > 2 * sms || kb < 2 * split)) break;
+    const double us = 4.0 + std::ceil(kb / split) * 0.37 * std::max(1.0, tiles * split / sms) +
+                      (i == 0 ? 0.0 : M > 16 ? kAdd[i] : 0.7);
+    if (i == 0 || us < best) {
+      best = us;
+      p.split = split;
+    }
+  }
+  const double pairs = std::ceil(double((M + 255) / 256) * double((N + 255) / 256) / (sms / 2));
+  p.pair = vec && 4.5 + pairs * (0.5 + 0.4 * kb) < best;
+  if (g_fp8_force_pair >= 0) p.pair = g_fp8_force_pair != 0;
+  return p;
 }
 
 template <typename T>
 void launch_linear_fp8(const void* A, int64_t lda, const void* As, const void* W, int64_t ldw, const void* Ws, T* C,
-                       int64_t ldc, int64_t M, int64_t N, int64_t K, const Epi<T>& epi, bool vec, bool pair,
-                       cudaStream_t s) {
+                       int64_t ldc, int64_t M, int64_t N, int64_t K, const Epi<T>& epi, bool vec, cudaStream_t s) {
+  const auto [pair, split] = fp8_plan(M, N, K, vec, num_sms());
   const CUtensorMap ta = make_tmap_u8_2d(A, uint64_t(K), uint64_t(M), uint64_t(lda), 128);
   const CUtensorMap tb = make_tmap_u8_2d(W, uint64_t(K), uint64_t(N), uint64_t(ldw), 128);
   const uint64_t quads = uint64_t(fp8_quads(K));
@@ -741,20 +810,9 @@ void launch_linear_fp8(const void* A, int64_t lda, const void* As, const void* W
   auto kern = gemm_fp8_tile_kernel<T>;
   ensure_smem_limit(smem_done[0], kern, Fp8TileCfg::SMEM);
   const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-  const int split = fp8_split(tiles, (K + 127) / 128);
   LTX_UNSUPPORTED(tiles * split < (int64_t(1) << 31), "too many tiles for one launch");
   launch_pdl(kern, dim3(unsigned(tiles * split)), dim3(192), Fp8TileCfg::SMEM, s, unsigned(split), ta, tb, tsa, tsb, C,
              ldc, int(M), int(N), int(K), split, int(vec), epi);
-}
-
-// Test hook (ltx_test_fp8_force_pair): -1 automatic, 0 single-CTA tiles, 1 CTA pairs.
-static thread_local int g_fp8_force_pair = -1;
-
-// CTA pairs from the size on at which their tiles keep most SMs busy (outputs that cannot
-// be stored 32 bytes at a time go through the tile kernel's staging).
-inline bool fp8_use_pair(int64_t M, int64_t N, bool vec) {
-  if (g_fp8_force_pair >= 0) return g_fp8_force_pair != 0;
-  return vec && ((M + 255) / 256) * ((N + 255) / 256) * 2 >= num_sms() / 2;
 }
 
 }  // namespace detail
@@ -945,7 +1003,7 @@ extern "C" int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, 
     bool vec;
     const Epi<T> e = make_epi_any<T>(epi, N, vec);
     vec = vec && reinterpret_cast<uintptr_t>(C) % 32 == 0 && ldc % 16 == 0;
-    launch_linear_fp8<T>(A, lda, a_scales, W, ldw, w_scales, cp, ldc, M, N, K, e, vec, fp8_use_pair(M, N, vec), s);
+    launch_linear_fp8<T>(A, lda, a_scales, W, ldw, w_scales, cp, ldc, M, N, K, e, vec, s);
   };
   if (dtype == LTX_F32)
     run(static_cast<float*>(C));
