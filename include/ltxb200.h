@@ -253,6 +253,14 @@ int ltx_norm_modulate_fp8(const void* x, int64_t ldx, void* q, int64_t ldq, void
 int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, const void* W, int64_t ldw, const void* w_scales,
                    void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, const ltx_epilogue* epi, int dtype,
                    void* stream);
+/* ltx_quantize_fp8 of x (M, K) in x_dtype, then ltx_linear_fp8, in one call: up to eight rows
+ * in one launch that quantises them while it streams W, more through the workspace (device
+ * memory, 16-byte aligned, ltx_quantize_linear_fp8_workspace_bytes(M, K) bytes, 0 when none is
+ * needed; no initialisation; calls that may run concurrently need one each). */
+size_t ltx_quantize_linear_fp8_workspace_bytes(int64_t M, int64_t K);
+int ltx_quantize_linear_fp8(const void* x, int64_t ldx, int x_dtype, const void* W, int64_t ldw, const void* w_scales,
+                            void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, const ltx_epilogue* epi,
+                            void* workspace, size_t workspace_bytes, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------- */
 /* Denoise update: X0 conversion + CFG guidance + Euler step.                          */

@@ -228,6 +228,10 @@ _SIGNATURES = {
                                              ctypes.c_float, ctypes.POINTER(Modulation), ctypes.c_int, c_vp]),
     "ltx_linear_fp8": (ctypes.c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
                                       ctypes.POINTER(Epilogue), ctypes.c_int, c_vp]),
+    "ltx_quantize_linear_fp8_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
+    "ltx_quantize_linear_fp8": (ctypes.c_int, [c_vp, c_i64, ctypes.c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                                               c_i64, ctypes.POINTER(Epilogue), c_vp, ctypes.c_size_t, ctypes.c_int,
+                                               c_vp]),
     "ltx_ctx_create": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(c_vp)]),
     "ltx_ctx_destroy": (ctypes.c_int, [c_vp]),
     "ltx_dit_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DitConfig), c_i64, c_i64]),
@@ -567,12 +571,12 @@ def attention_merge(o_parts: torch.Tensor, lse_parts: torch.Tensor, gate_logits:
 def _on(t: torch.Tensor, name: str, *args, label: str | None = None) -> None:
     """_call with the stream of t's device appended, made on that device (which need not be
     the current one)."""
-    dev = t.device
-    if dev.index == torch.cuda.current_device():
-        _call(name, *args, torch.cuda.current_stream(dev).cuda_stream, label=label)
+    dev = t.device.index
+    if dev == torch.cuda.current_device():
+        _call(name, *args, torch._C._cuda_getCurrentRawStream(dev), label=label)
         return
     with torch.cuda.device(dev):
-        _call(name, *args, torch.cuda.current_stream(dev).cuda_stream, label=label)
+        _call(name, *args, torch._C._cuda_getCurrentRawStream(dev), label=label)
 
 
 def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
@@ -679,6 +683,24 @@ def linear_fp8(a: Fp8Rows, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = N
 def fp8_force_pair(pair: int) -> None:
     """Test hook (include/ltxb200_testing.h): force the calling thread's linear_fp8 kernel."""
     _call("ltx_test_fp8_force_pair", pair)
+
+
+def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = None) -> None:
+    """c = epilogue(quantize_fp8(x) @ w.T (+ bias)); x (M, K) float32 or bfloat16 with unit
+    column stride, c (M, N) a row-major view in the epilogue's type."""
+    m, k = x.shape
+    if k != w.cols or tuple(c.shape) != (m, w.rows):
+        raise ValueError(f"shape mismatch x{tuple(x.shape)} w{w.shape} c{tuple(c.shape)}")
+    xdt, ldx, dt, ld = _dt(x), _ld(x), _dt(c), _ld(c)
+    _same_device(x, c, w.data)
+    if not c.numel():
+        return
+    n = load_library().ltx_quantize_linear_fp8_workspace_bytes(m, k)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _on(x, "ltx_quantize_linear_fp8", x.data_ptr(), ldx, xdt, w.data.data_ptr(), w.data.stride(0), w.scales.data_ptr(),
+        c.data_ptr(), ld, m, w.rows, k, ctypes.byref(epi) if epi is not None else None,
+        ws.data_ptr() if n else None, n, dt,
+        label=f"quantize_linear_fp8 M={m} N={w.rows} K={k}" if _profile is not None else None)
 
 
 MASK_KINDS = {torch.bool: 0, torch.float32: 1, torch.bfloat16: 2}

@@ -2,6 +2,7 @@
 //   ltx_quantize_fp8, ltx_dequantize_fp8, ltx_fp8_pack_scales   the format
 //   ltx_norm_modulate_fp8   norm + adaLN modulation written as 8-bit rows
 //   ltx_linear_fp8          C = epilogue(A W^T), A and W 8-bit rows
+//   ltx_quantize_linear_fp8 the same from F32 / BF16 rows
 // None has a counterpart in the reference, which runs its linear layers in bf16
 // (ltx_nn.py:126-158, 188-192, 244-245).
 #include <algorithm>
@@ -815,6 +816,159 @@ void launch_linear_fp8(const void* A, int64_t lda, const void* As, const void* W
              ldc, int(M), int(N), int(K), split, int(vec), epi);
 }
 
+// ---------------------------------------------------------------------------------
+// One to eight rows (adaLN: one row per sample): the product is reading W once. One launch
+// quantises the rows in every CTA (M * K values, from L2) and streams W through registers:
+// a CTA takes 16 rows of W at a time, warp w of 8 the blocks w, w + 8, .. of 128 columns, so
+// that a group's bytes are in flight at once; each block is four warp-level MMAs (16 rows of
+// W by 8 of x, K = 32) from zero, and the sums are multiplied by both scales and added in
+// fp32. A dot product does not depend on the order of its terms, so lane l feeds the MMAs
+// the 32 contiguous bytes l % 4 of its rows' 128 (the same of W and of x). The eight warps'
+// sums are added in order through shared memory. CUDA-core products, two rows of W per
+// warp, took 14.3 us at 2 x 12288 x 2048 (unpacking e4m3 bounds them) and the tile kernel 13.
+// ---------------------------------------------------------------------------------
+LTX_DEVICE void mma_e4m3_16x8x32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                 uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kFp8RowsMax = 8;
+
+// 32 bytes of a row of W from column c on, zeros from K on (the row's padding may hold any
+// byte, and must not meet the MMA as NaN). wide: 32-byte aligned rows.
+LTX_DEVICE void fp8_load_w32(const uint8_t* row, int c, int K, bool wide, uint32_t (&v)[8]) {
+  if (wide && c + 32 <= K) {
+    ldg_32b(row + c, v);
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = c + 16 * h;
+    const uint4 u = at < K ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+    const uint32_t b[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int left = K - at - 4 * i;  // bytes of this word that exist
+      v[4 * h + i] = left >= 4 ? b[i] : left <= 0 ? 0u : b[i] & ((1u << (8 * left)) - 1u);
+    }
+  }
+}
+
+template <typename T, typename X>
+__global__ void __launch_bounds__(256, 2)
+    linear_fp8_rows_kernel(const X* __restrict__ x, int64_t ldx, int vec_x, const uint8_t* __restrict__ W, int64_t ldw,
+                           int wide, const uint32_t* __restrict__ Ws, int64_t w_padded, T* __restrict__ C, int64_t ldc,
+                           int M, int N, int K, Epi<T> epi) {
+  extern __shared__ __align__(16) uint8_t rows_smem[];
+  __shared__ float part[2][8][16][kFp8RowsMax];
+  const int quads = (K + kFp8Quad - 1) / kFp8Quad, blocks = (K + kFp8Block - 1) / kFp8Block;
+  const int ldxq = quads * kFp8Quad + 16;                             // no bank conflicts between rows
+  float* sa = reinterpret_cast<float*>(rows_smem + M * ldxq);         // [M][quads * 4]
+  const int lane = lane_id(), warp = warp_id(), row = lane >> 2, piece = lane & 3;
+  pdl_wait();
+  pdl_trigger();
+
+  constexpr int PRE = 2;  // blocks per warp in flight
+  uint32_t w[PRE][2][8], sw[PRE][2];
+  // blocks warp + 8 i, i in [i0, i0 + PRE), of the 16 rows from n0 on
+  auto fetch = [&](int n0, int i0) {
+#pragma unroll
+    for (int j = 0; j < PRE; ++j) {
+      const int kb = warp + 8 * (i0 + j);
+      if (kb >= blocks) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t n = min(n0 + row + 8 * h, N - 1);
+        fp8_load_w32(W + n * ldw, kb * kFp8Block + piece * 32, K, wide, w[j][h]);
+        sw[j][h] = Ws[fp8_word(n, kb >> 2, w_padded)];
+      }
+    }
+  };
+  int n0 = blockIdx.x * 16;
+  fetch(n0, 0);
+  for (int i = warp; i < M * quads; i += 8) {
+    const int m = i / quads, kq = i - m * quads;
+    float v[16];
+    load16<X>(x + m * ldx, kq * kFp8Quad + lane * 16, K, vec_x, v);
+    uint4 q;
+    const int code = fp8_quantize16(v, q);
+    *reinterpret_cast<uint4*>(rows_smem + m * ldxq + kq * kFp8Quad + lane * 16) = q;
+    if ((lane & 7) == 0) sa[i * 4 + (lane >> 3)] = fp8_scale(code);
+  }
+  __syncthreads();
+  const int per_warp = (blocks - warp + 7) / 8;
+  for (int buf = 0; n0 < N; n0 += int(gridDim.x) * 16, buf ^= 1) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < per_warp; i0 += PRE) {
+#pragma unroll
+      for (int j = 0; j < PRE; ++j) {
+        const int kb = warp + 8 * (i0 + j);
+        if (kb >= blocks) break;
+        uint32_t b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (row < M) {
+          const uint4* p = reinterpret_cast<const uint4*>(rows_smem + row * ldxq + kb * kFp8Block + piece * 32);
+          const uint4 u0 = p[0], u1 = p[1];
+          b[0] = u0.x; b[1] = u0.y; b[2] = u0.z; b[3] = u0.w;
+          b[4] = u1.x; b[5] = u1.y; b[6] = u1.z; b[7] = u1.w;
+        }
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < 8; t += 2)
+          mma_e4m3_16x8x32(c, w[j][0][t], w[j][1][t], w[j][0][t + 1], w[j][1][t + 1], b[t], b[t + 1]);
+        // c: (W row `row`, x rows 2 piece and 2 piece + 1), then the same of W row `row` + 8
+        const float a0 = 2 * piece < M ? sa[2 * piece * quads * 4 + kb] : 0.f;
+        const float a1 = 2 * piece + 1 < M ? sa[(2 * piece + 1) * quads * 4 + kb] : 0.f;
+        const float s0 = fp8_scale((sw[j][0] >> (8 * (kb & 3))) & 255u);
+        const float s1 = fp8_scale((sw[j][1] >> (8 * (kb & 3))) & 255u);
+        acc[0] = fmaf(c[0] * a0, s0, acc[0]);
+        acc[1] = fmaf(c[1] * a1, s0, acc[1]);
+        acc[2] = fmaf(c[2] * a0, s1, acc[2]);
+        acc[3] = fmaf(c[3] * a1, s1, acc[3]);
+      }
+      if (i0 + PRE < per_warp) fetch(n0, i0 + PRE);
+    }
+    const int next = n0 + int(gridDim.x) * 16;
+    if (next < N) fetch(next, 0);
+    *reinterpret_cast<float2*>(&part[buf][warp][row][2 * piece]) = make_float2(acc[0], acc[1]);
+    *reinterpret_cast<float2*>(&part[buf][warp][row + 8][2 * piece]) = make_float2(acc[2], acc[3]);
+    __syncthreads();  // the other buffer is rewritten only behind the next one
+    for (int i = threadIdx.x; i < 16 * M; i += 256) {
+      const int m = i >> 4, r = i & 15;
+      if (n0 + r < N) {
+        float v[1] = {0.f};
+#pragma unroll
+        for (int p = 0; p < 8; ++p) v[0] += part[buf][p][r][m];
+        const int64_t sb = m / epi.rows_per_batch, st = m - sb * epi.rows_per_batch;
+        fp8_epilogue<T, 1>(epi, C + m * ldc, m, sb, st, n0 + r, v);
+      }
+    }
+  }
+}
+
+inline int64_t fp8_rows_smem(int64_t M, int64_t K) { return M * (fp8_quads(K) * (512 + 16) + 16); }
+// The streaming kernel, as long as two CTAs' quantised rows fit in an SM's shared memory.
+inline bool fp8_use_rows(int64_t M, int64_t K) {
+  return M <= kFp8RowsMax && fp8_rows_smem(M, K) <= 96 * 1024 && g_fp8_force_pair < 0;
+}
+
+template <typename T, typename X>
+void launch_fp8_rows(const X* x, int64_t ldx, const void* W, int64_t ldw, const void* Ws, T* C, int64_t ldc, int64_t M,
+                     int64_t N, int64_t K, const Epi<T>& epi, cudaStream_t s) {
+  const int smem = int(fp8_rows_smem(M, K));
+  auto kern = linear_fp8_rows_kernel<T, X>;
+  static std::atomic<uint64_t> smem_done{0};
+  ensure_smem_limit(smem_done, kern, 96 * 1024);
+  const int64_t grid = std::min<int64_t>((N + 15) / 16, int64_t(num_sms()) * 2);
+  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+  const int wide = reinterpret_cast<uintptr_t>(W) % 32 == 0 && ldw % 32 == 0;
+  launch_pdl(kern, dim3(unsigned(grid)), dim3(256), size_t(smem), s, 1, x, ldx, vec, static_cast<const uint8_t*>(W), ldw,
+             wide, static_cast<const uint32_t*>(Ws), fp8_rows_padded(N), C, ldc, int(M), int(N), int(K), epi);
+}
+
 }  // namespace detail
 }  // namespace ltx
 
@@ -898,15 +1052,8 @@ extern "C" size_t ltx_fp8_scale_bytes(int64_t rows, int64_t cols) {
   return size_t(fp8_rows_padded(rows)) * size_t(fp8_quads(cols)) * 4;
 }
 
-extern "C" int ltx_quantize_fp8(const void* x, int64_t ldx, int64_t rows, int64_t cols, void* q, int64_t ldq,
-                                void* scales, int dtype, void* stream) {
-  LTX_API_BEGIN
-  LTX_REQUIRE(dtype == LTX_F32 || dtype == LTX_BF16, "dtype must be F32 or BF16");
-  LTX_REQUIRE(x != nullptr, "x must be non-NULL");
-  check_fp8_rows(q, ldq, scales, rows, cols, "ltx_quantize_fp8: output");
-  LTX_REQUIRE(ldx >= cols, "ldx must hold the columns");
-  LTX_REQUIRE(reinterpret_cast<uintptr_t>(x) % (dtype == LTX_F32 ? 4 : 2) == 0, "x is not aligned to its type");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
+static void launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, void* q, int64_t ldq, void* scales,
+                            int dtype, cudaStream_t s) {
   const int quads = int(fp8_quads(cols));
   const unsigned grid = grid_for((rows * quads + 7) / 8);
   const int vec = vec_ok(x, ldx);
@@ -918,6 +1065,17 @@ extern "C" int ltx_quantize_fp8(const void* x, int64_t ldx, int64_t rows, int64_
     run(static_cast<const float*>(x), quantize_fp8_kernel<float>);
   else
     run(static_cast<const __nv_bfloat16*>(x), quantize_fp8_kernel<__nv_bfloat16>);
+}
+
+extern "C" int ltx_quantize_fp8(const void* x, int64_t ldx, int64_t rows, int64_t cols, void* q, int64_t ldq,
+                                void* scales, int dtype, void* stream) {
+  LTX_API_BEGIN
+  LTX_REQUIRE(dtype == LTX_F32 || dtype == LTX_BF16, "dtype must be F32 or BF16");
+  LTX_REQUIRE(x != nullptr, "x must be non-NULL");
+  check_fp8_rows(q, ldq, scales, rows, cols, "ltx_quantize_fp8: output");
+  LTX_REQUIRE(ldx >= cols, "ldx must hold the columns");
+  LTX_REQUIRE(reinterpret_cast<uintptr_t>(x) % (dtype == LTX_F32 ? 4 : 2) == 0, "x is not aligned to its type");
+  launch_quantize(x, ldx, rows, cols, q, ldq, scales, dtype, static_cast<cudaStream_t>(stream));
   LTX_API_END
 }
 
@@ -1010,6 +1168,62 @@ extern "C" int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, 
   else
     run(static_cast<__nv_bfloat16*>(C));
   LTX_CUDA(cudaGetLastError());
+  LTX_API_END
+}
+
+// Workspace of ltx_quantize_linear_fp8: the quantised rows' data, then their scales.
+static size_t quantized_data_bytes(int64_t M, int64_t K) { return size_t(M) * size_t((K + 15) / 16 * 16); }
+
+extern "C" size_t ltx_quantize_linear_fp8_workspace_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || fp8_use_rows(M, K)) return 0;
+  return (quantized_data_bytes(M, K) + 15) / 16 * 16 + ltx_fp8_scale_bytes(M, K);
+}
+
+extern "C" int ltx_quantize_linear_fp8(const void* x, int64_t ldx, int x_dtype, const void* W, int64_t ldw,
+                                       const void* w_scales, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K,
+                                       const ltx_epilogue* epi, void* workspace, size_t workspace_bytes, int dtype,
+                                       void* stream) {
+  LTX_API_BEGIN
+  LTX_REQUIRE(dtype == LTX_F32 || dtype == LTX_BF16, "dtype must be F32 or BF16");
+  LTX_REQUIRE(x_dtype == LTX_F32 || x_dtype == LTX_BF16, "x_dtype must be F32 or BF16");
+  LTX_REQUIRE(x != nullptr && C != nullptr, "x and C must be non-NULL");
+  LTX_REQUIRE(M > 0 && N > 0 && K > 0, "M, N, K must be positive");
+  LTX_REQUIRE(M < (int64_t(1) << 31) - 256, "size out of range");
+  check_fp8_rows(W, ldw, w_scales, N, K, "ltx_quantize_linear_fp8: W");
+  LTX_REQUIRE(ldx >= K, "ldx must hold the columns");
+  LTX_REQUIRE(ldc >= N, "ldc must hold the columns");
+  LTX_REQUIRE(reinterpret_cast<uintptr_t>(x) % (x_dtype == LTX_F32 ? 4 : 2) == 0, "x is not aligned to its type");
+  LTX_REQUIRE(reinterpret_cast<uintptr_t>(C) % (dtype == LTX_F32 ? 4 : 2) == 0, "C is not aligned to its type");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!fp8_use_rows(M, K)) {
+    LTX_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                    workspace_bytes >= ltx_quantize_linear_fp8_workspace_bytes(M, K),
+                "the workspace must be 16-byte aligned and hold ltx_quantize_linear_fp8_workspace_bytes(M, K) bytes");
+    const int64_t ldq = (K + 15) / 16 * 16;
+    void* scales = static_cast<char*>(workspace) + (quantized_data_bytes(M, K) + 15) / 16 * 16;
+    bool unused;  // the epilogue is checked before the first launch
+    if (dtype == LTX_F32)
+      make_epi_any<float>(epi, N, unused);
+    else
+      make_epi_any<__nv_bfloat16>(epi, N, unused);
+    launch_quantize(x, ldx, M, K, workspace, ldq, scales, x_dtype, s);
+    return ltx_linear_fp8(workspace, ldq, scales, W, ldw, w_scales, C, ldc, M, N, K, epi, dtype, stream);
+  }
+  auto run = [&](auto* xp, auto* cp) {
+    using T = std::remove_pointer_t<decltype(cp)>;
+    bool unused;
+    launch_fp8_rows(xp, ldx, W, ldw, w_scales, cp, ldc, M, N, K, make_epi_any<T>(epi, N, unused), s);
+  };
+  auto run_c = [&](auto* xp) {
+    if (dtype == LTX_F32)
+      run(xp, static_cast<float*>(C));
+    else
+      run(xp, static_cast<__nv_bfloat16*>(C));
+  };
+  if (x_dtype == LTX_F32)
+    run_c(static_cast<const float*>(x));
+  else
+    run_c(static_cast<const __nv_bfloat16*>(x));
   LTX_API_END
 }
 

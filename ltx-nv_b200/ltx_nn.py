@@ -242,10 +242,13 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
         out = torch.empty(shape, device=x.device, dtype=dtype)
     elif not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    rows = x if isinstance(x, Fp8Rows) else quantize_fp8(x)
-    nat.linear_fp8(rows, weight, out.view(-1, n),
-                   nat.epilogue(kind, bias=bias.contiguous() if bias is not None else None,
-                                residual=residual2 if residual is not None else None, gate=mod, rows_per_batch=rpb))
+    epi = nat.epilogue(kind, bias=bias.contiguous() if bias is not None else None,
+                       residual=residual2 if residual is not None else None, gate=mod, rows_per_batch=rpb)
+    if isinstance(x, Fp8Rows):
+        nat.linear_fp8(x, weight, out.view(-1, n), epi)
+    elif weight.cols:
+        x2 = x.reshape(-1, weight.cols)
+        nat.quantize_linear_fp8(x2 if x2.stride(1) == 1 else x2.contiguous(), weight, out.view(-1, n), epi)
     return out
 
 

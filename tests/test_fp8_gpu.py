@@ -192,7 +192,8 @@ def check(got, want, slack, dtype):
     assert rel <= HALF[dtype] + 2e-6, rel
 
 
-SHAPES = [(1, 1, 1), (1, 8, 16), (2, 12288, 2048), (3, 5, 100), (31, 256, 128), (32, 128, 129), (33, 300, 512),
+SHAPES = [(1, 1, 1), (1, 8, 16), (2, 12288, 2048), (3, 5, 100), (4, 33, 1200), (5, 5000, 999), (7, 17, 8200),
+          (8, 2000, 4097), (6, 24, 20000), (9, 40, 600), (31, 256, 128), (32, 128, 129), (33, 300, 512),
           (100, 72, 4096), (127, 129, 130), (128, 128, 1024), (129, 257, 640), (252, 6176, 2048), (256, 512, 513),
           (257, 1371, 1037), (300, 2048, 8192), (1000, 96, 64), (1025, 776, 1536), (2048, 2304, 256),
           (3000, 4100, 384), (2560, 5120, 1040)]  # more than one tile per SM pair
