@@ -13,10 +13,55 @@
 namespace ltx {
 namespace detail {
 
-// 16 consecutive columns [c, c + 16) of a row, zeros from `cols` on. `vec`: the row is
-// 16-byte aligned and whole groups of 8 columns may be loaded at once.
+// 16 consecutive values, 32 (bf16) or 64 (fp32) bytes, 32-byte aligned.
+template <typename T> LTX_DEVICE void ld16v(const T* p, float (&v)[16]);
+template <> LTX_DEVICE void ld16v<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[16]) {
+  uint32_t r[8];
+  ldg_32b(p, r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) unpack_bf16x2(r[i], v[2 * i], v[2 * i + 1]);
+}
+template <> LTX_DEVICE void ld16v<float>(const float* p, float (&v)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r[8];
+    ldg_32b(p + 8 * h, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(r[i]);
+  }
+}
+template <typename T> LTX_DEVICE void st16v(T* p, const float (&v)[16]);
+template <> LTX_DEVICE void st16v<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[16]) {
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  stg_32b(p, r);
+}
+template <> LTX_DEVICE void st16v<float>(float* p, const float (&v)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[8 * h + i]);
+    stg_32b(p + 8 * h, r);
+  }
+}
+
+// How the rows of an operand may be read: 0 by element, 1 by 16 bytes, 2 by 32 bytes.
 template <typename T>
-LTX_DEVICE void load16(const T* row, int64_t c, int64_t cols, bool vec, float (&v)[16]) {
+inline int row_vec(const T* p, int64_t ld) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const int64_t b = ld * int64_t(sizeof(T));
+  return a % 32 == 0 && b % 32 == 0 ? 2 : a % 16 == 0 && b % 16 == 0 && ld % 8 == 0 ? 1 : 0;
+}
+
+// 16 consecutive columns [c, c + 16) of a row, zeros from `cols` on.
+template <typename T>
+LTX_DEVICE void load16(const T* row, int64_t c, int64_t cols, int vec, float (&v)[16]) {
+  if (vec == 2 && c + 16 <= cols) {
+    ld16v<T>(row + c, v);
+    return;
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t c8 = c + 8 * h;
@@ -32,12 +77,14 @@ LTX_DEVICE void load16(const T* row, int64_t c, int64_t cols, bool vec, float (&
   }
 }
 
-// One warp per (row, 512 columns): two 16-byte loads and one 16-byte store per lane.
+// A warp per (row, 512 columns): 32 bytes (bf16) per lane in, 16 out. HBM-bound: 47.5 us at
+// 12288 x 8192 bf16 = 6.4 TB/s, 97 % of the measured copy. Many short warps per SM keep
+// more bytes in flight than several rows per warp (two rows 65 us, four 98).
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
-                                                           int64_t cols, int quads, int vec,
-                                                           uint8_t* __restrict__ q, int64_t ldq,
-                                                           uint32_t* __restrict__ scales, int64_t rows_padded) {
+__global__ void __launch_bounds__(256, 6) quantize_fp8_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
+                                                              int64_t cols, int quads, int vec,
+                                                              uint8_t* __restrict__ q, int64_t ldq,
+                                                              uint32_t* __restrict__ scales, int64_t rows_padded) {
   pdl_wait();
   pdl_trigger();
   const int64_t task = int64_t(blockIdx.x) * 8 + warp_id();
@@ -49,39 +96,53 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__
   load16<T>(x + r * ldx, c, cols, vec, v);
   uint4 out;
   const int code = fp8_quantize16(v, out);
-  const uint32_t word = fp8_quad_word(code);
   if (c < cols) *reinterpret_cast<uint4*>(q + r * ldq + c) = out;
-  if (lane_id() == 0) scales[fp8_word(r, kq, rows_padded)] = word;
+  fp8_store_codes(scales + fp8_word(r, kq, rows_padded), code);
 }
 
-// One thread per 8 columns.
+constexpr int kDequantRows = 4;
+// A warp takes 512 columns of four rows, all of whose loads are in flight together.
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_fp8_kernel(const uint8_t* __restrict__ q, int64_t ldq,
                                                              const uint32_t* __restrict__ scales, int64_t rows_padded,
-                                                             int64_t rows, int64_t cols, int vec, T* __restrict__ x,
-                                                             int64_t ldx) {
+                                                             int64_t rows, int64_t cols, int quads, int vec,
+                                                             T* __restrict__ x, int64_t ldx) {
   pdl_wait();
   pdl_trigger();
-  const int64_t per_row = (cols + 7) / 8;
-  const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= rows * per_row) return;
-  const int64_t r = i / per_row, c = (i - r * per_row) * 8;
-  const uint32_t word = scales[fp8_word(r, c / kFp8Quad, rows_padded)];
-  const float s = fp8_scale((word >> (8 * ((c / kFp8Block) & 3))) & 255);
-  const uint2 w = *reinterpret_cast<const uint2*>(q + r * ldq + c);  // ldq % 16 == 0: in the padded row
-  float v[8];
-  fp8_unpack2(w.x, v[0], v[1]);
-  fp8_unpack2(w.x >> 16, v[2], v[3]);
-  fp8_unpack2(w.y, v[4], v[5]);
-  fp8_unpack2(w.y >> 16, v[6], v[7]);
+  const int64_t task = int64_t(blockIdx.x) * 8 + warp_id();
+  const int64_t r0 = task / quads * kDequantRows;
+  const int kq = int(task % quads);
+  const int64_t c = int64_t(kq) * kFp8Quad + lane_id() * 16;
+  if (r0 >= rows || c >= cols) return;
+  uint4 w[kDequantRows];
+  uint32_t word[kDequantRows];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] *= s;
-  if (vec && c + 8 <= cols) {
-    st8<T>(x + r * ldx + c, v);
-  } else {
+  for (int i = 0; i < kDequantRows; ++i) {
+    const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
+    w[i] = *reinterpret_cast<const uint4*>(q + r * ldq + c);  // inside the row: ldq is a multiple of 16
+    word[i] = scales[fp8_word(r, kq, rows_padded)];
+  }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < cols) st_elem<T>(x + r * ldx + c + k, v[k]);
+  for (int i = 0; i < kDequantRows; ++i) {
+    if (r0 + i >= rows) break;
+    const float s = fp8_scale((word[i] >> (8 * (lane_id() >> 3))) & 255);
+    const uint32_t b[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      fp8_unpack2(b[j], v[4 * j], v[4 * j + 1]);
+      fp8_unpack2(b[j] >> 16, v[4 * j + 2], v[4 * j + 3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= s;
+    T* row = x + (r0 + i) * ldx;
+    if (vec == 2 && c + 16 <= cols) {
+      st16v<T>(row + c, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c + j < cols) st_elem<T>(row + c + j, v[j]);
+    }
   }
 }
 
@@ -123,57 +184,154 @@ LTX_DEVICE void modvec8(const ModVec<T>& m, int64_t b, int64_t t, int64_t c, flo
   }
 }
 
-// y = norm(x) * (1 + scale) + shift in fp32, quantised once. One CTA per row, one warp
-// per 512 columns, 16 columns per lane.
+// Modulation vectors of this lane's 16 columns as pairs: 1 + scale and shift.
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_modulate_fp8_kernel(const T* __restrict__ x, int64_t ldx,
-                                                                 int64_t rows_per_batch, int D, int kind, float eps,
-                                                                 ModVec<T> shift, ModVec<T> scale,
-                                                                 uint8_t* __restrict__ q, int64_t ldq,
-                                                                 uint32_t* __restrict__ scales, int64_t rows_padded) {
-  __shared__ float red[32];
-  pdl_wait();
-  pdl_trigger();
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / rows_per_batch, t = row - b * rows_per_batch;
-  const int c = threadIdx.x * 16;
-  float v[16];
-  load16<T>(x + row * ldx, c, D, true, v);
-  float mean = 0.f, rstd = 1.f;
-  if (kind != LTX_NORM_NONE) {
-    if (kind == LTX_NORM_LAYER) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s += v[i];
-      mean = block_sum(s, red) / float(D);
-    }
-    float s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float d = c + i < D ? v[i] - mean : 0.f;
-      s2 = fmaf(d, d, s2);
-    }
-    rstd = 1.f / sqrtf(block_sum(s2, red) / float(D) + eps);
-  }
+LTX_DEVICE void norm_vectors(const ModVec<T>& scale, const ModVec<T>& shift, int64_t b, int64_t t, int c, int D,
+                             uint64_t (&sc)[8], uint64_t (&sh)[8]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float sc[8], sh[8];
-    const bool in = c + 8 * h < D;
+    float a[8], e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sc[i] = sh[i] = 0.f;
-    if (in && scale.on) modvec8<T>(scale, b, t, c + 8 * h, sc);
-    if (in && shift.on) modvec8<T>(shift, b, t, c + 8 * h, sh);
+    for (int i = 0; i < 8; ++i) a[i] = e[i] = 0.f;
+    if (scale.on && c + 8 * h < D) modvec8<T>(scale, b, t, c + 8 * h, a);
+    if (shift.on && c + 8 * h < D) modvec8<T>(shift, b, t, c + 8 * h, e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = (v[8 * h + i] - mean) * rstd;
-      v[8 * h + i] = in ? fmaf(y, 1.f + sc[i], sh[i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      sc[4 * h + i] = f2_pack(1.f + a[2 * i], 1.f + a[2 * i + 1]);
+      sh[4 * h + i] = f2_pack(e[2 * i], e[2 * i + 1]);
     }
   }
-  uint4 out;
-  const int code = fp8_quantize16(v, out);
-  const uint32_t word = fp8_quad_word(code);
-  if (c < D) *reinterpret_cast<uint4*>(q + row * ldq + c) = out;
-  if (lane_id() == 0) scales[fp8_word(row, warp_id(), rows_padded)] = word;
+}
+
+// Sixteen columns as loaded: raw bits, so that a prefetched bf16 row costs 8 registers.
+template <typename T>
+struct Raw16 {
+  static constexpr int N = 4 * int(sizeof(T));
+  uint32_t r[N];
+  LTX_DEVICE void load(const T* row, int c, int cols, int vec) {
+    if (vec == 2 && c + 16 <= cols) {
+#pragma unroll
+      for (int h = 0; h < N / 8; ++h) {
+        uint32_t t[8];
+        ldg_32b(reinterpret_cast<const uint8_t*>(row + c) + 32 * h, t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[8 * h + i] = t[i];
+      }
+      return;
+    }
+#pragma unroll
+    for (int h = 0; h < N / 4; ++h) {  // columns are a multiple of 8: 16-byte pieces are whole
+      const int at = c + h * (16 / int(sizeof(T)));
+      const uint4 u = at < cols ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+      r[4 * h] = u.x; r[4 * h + 1] = u.y; r[4 * h + 2] = u.z; r[4 * h + 3] = u.w;
+    }
+  }
+  LTX_DEVICE void get(uint64_t (&v)[8]) const {  // fp32 pairs
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 2)
+        v[i] = f2_pack(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u));
+      else
+        v[i] = f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    }
+  }
+};
+
+// y = norm(x) * (1 + scale) + shift in fp32, quantised once. A row takes `wr` warps, 512
+// columns each, 16 per lane; a CTA holds groups = 8 / wr rows at a time (wr <= 8) and walks
+// `per_cta` rows of one sample, whose vectors stay in registers (HOIST: per-sample vectors
+// and rows of at most 8192 columns). The next row is loaded before this one is reduced: one
+// __syncthreads per row (two for LayerNorm, whose squares are taken about the mean).
+// 12288 x 2048 bf16: 19.9 us = 3.8 TB/s, 58 % of the measured copy, bound by instruction
+// issue (65 % active, 330 instructions per 512 columns before the packed arithmetic); rows
+// with their vectors reloaded took 49 us, a deeper prefetch changed nothing.
+template <typename T, int KIND, bool HOIST, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
+    norm_modulate_fp8_kernel(const T* __restrict__ x, int64_t ldx, int vec, int64_t rows, int64_t rows_per_batch, int D,
+                             int wr, int chunks, int per_cta, float eps, ModVec<T> shift, ModVec<T> scale,
+                             uint8_t* __restrict__ q, int64_t ldq, uint32_t* __restrict__ scales,
+                             int64_t rows_padded) {
+  __shared__ float red[4][32];
+  const int groups = int(blockDim.x >> 5) / wr, group = warp_id() / wr, w = warp_id() - group * wr;
+  const int c = (w * 32 + lane_id()) * 16;
+  // rows [r0, r1) of sample b; this group's are r0 + group, step groups
+  const int64_t b = blockIdx.x / chunks;
+  const int64_t r0 = b * rows_per_batch + int64_t(blockIdx.x - b * chunks) * per_cta;
+  const int64_t r1 = min(min(r0 + per_cta, (b + 1) * rows_per_batch), rows);
+  pdl_wait();
+  pdl_trigger();
+  Raw16<T> raw;
+  if (r0 + group < r1) raw.load(x + (r0 + group) * ldx, c, D, vec);
+  uint64_t sc[8], sh[8];
+  if constexpr (HOIST) norm_vectors<T>(scale, shift, b, 0, c, D, sc, sh);
+  const bool whole = c + 16 <= D;  // all of this lane's columns exist
+  const float inv_d = 1.f / float(D);
+  int phase = 0;
+  // Sum over the row's warps, in warp order (the same value in all of them).
+  auto row_sum = [&](float s) {
+    s = warp_sum(s);
+    if (wr > 1) {
+      if (lane_id() == 0) red[phase][warp_id()] = s;
+      __syncthreads();
+      s = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < wr; ++i) s += red[phase][group * wr + i];
+      phase = (phase + 1) & 3;  // a buffer is written again three barriers later
+    }
+    return s;
+  };
+  for (int64_t base = r0; base < r1; base += groups) {  // the same count for every thread
+    const int64_t row = base + group;
+    uint64_t v[8];
+    raw.get(v);
+    if (row + groups < r1) raw.load(x + (row + groups) * ldx, c, D, vec);
+    auto total = [](const uint64_t (&t)[4]) {
+      float lo, hi;
+      f2_unpack(f2_add(f2_add(t[0], t[1]), f2_add(t[2], t[3])), lo, hi);
+      return lo + hi;
+    };
+    // columns past D hold zeros and stay zeros
+    auto clear = [&]() {
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + 2 * i >= D) v[i] = 0;
+      }
+    };
+    if constexpr (KIND == LTX_NORM_LAYER) {
+      uint64_t t[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+      for (int i = 4; i < 8; ++i) t[i - 4] = f2_add(t[i - 4], v[i]);
+      const float mean = row_sum(total(t)) * inv_d;
+      const uint64_t m2 = f2_pack(mean, mean);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = f2_sub(v[i], m2);
+      clear();
+    }
+    if constexpr (KIND != LTX_NORM_NONE) {
+      uint64_t t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = f2_fma(v[i + 4], v[i + 4], f2_mul(v[i], v[i]));
+      // one Newton step on the approximate root: within an ulp
+      const float a = fmaf(row_sum(total(t)), inv_d, eps), y = rsqrtf(a);
+      const float rstd = a > 0.f && a < __int_as_float(0x7f800000) ? y * fmaf(-0.5f * a * y, y, 1.5f) : y;
+      const uint64_t r2 = f2_pack(rstd, rstd);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = f2_mul(v[i], r2);
+    }
+    if (row >= r1) continue;  // uniform over the row's warps
+    if constexpr (!HOIST) norm_vectors<T>(scale, shift, b, row - b * rows_per_batch, c, D, sc, sh);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f2_fma(v[i], sc[i], sh[i]);
+    clear();
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f2_unpack(v[i], y[2 * i], y[2 * i + 1]);
+    uint4 out;
+    const int code = fp8_quantize16(y, out);
+    if (c < D) *reinterpret_cast<uint4*>(q + row * ldq + c) = out;
+    fp8_store_codes(scales + fp8_word(row, w, rows_padded), code);
+  }
 }
 
 // GELU (tanh form) as v * sigmoid(2 z), z = sqrt(2/pi) (v + 0.044715 v^3): one exponential
@@ -201,40 +359,6 @@ template <> LTX_DEVICE void st4v<__nv_bfloat16>(__nv_bfloat16* p, const float (&
 template <> LTX_DEVICE void st4v<float>(float* p, const float (&v)[4]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
-// 16 consecutive values, 32 (bf16) or 64 (fp32) bytes, 32-byte aligned.
-template <typename T> LTX_DEVICE void ld16v(const T* p, float (&v)[16]);
-template <> LTX_DEVICE void ld16v<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[16]) {
-  uint32_t r[8];
-  ldg_32b(p, r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) unpack_bf16x2(r[i], v[2 * i], v[2 * i + 1]);
-}
-template <> LTX_DEVICE void ld16v<float>(const float* p, float (&v)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t r[8];
-    ldg_32b(p + 8 * h, r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * h + i] = __uint_as_float(r[i]);
-  }
-}
-template <typename T> LTX_DEVICE void st16v(T* p, const float (&v)[16]);
-template <> LTX_DEVICE void st16v<__nv_bfloat16>(__nv_bfloat16* p, const float (&v)[16]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-  stg_32b(p, r);
-}
-template <> LTX_DEVICE void st16v<float>(float* p, const float (&v)[16]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t r[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[8 * h + i]);
-    stg_32b(p + 8 * h, r);
-  }
-}
-
 // Epilogue of W (1, 4 or 16) accumulators, columns [col, col + W) of row `row` (sample sb, token
 // st), in fp32 and rounded once on the store: acc + bias, then the activation, residual +
 // gate * (acc + bias), or + row_vec on marked rows. W > 1 needs every vector aligned there.
@@ -963,7 +1087,7 @@ void launch_fp8_rows(const X* x, int64_t ldx, const void* W, int64_t ldw, const 
   static std::atomic<uint64_t> smem_done{0};
   ensure_smem_limit(smem_done, kern, 96 * 1024);
   const int64_t grid = std::min<int64_t>((N + 15) / 16, int64_t(num_sms()) * 2);
-  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+  const int vec = row_vec(x, ldx);
   const int wide = reinterpret_cast<uintptr_t>(W) % 32 == 0 && ldw % 32 == 0;
   launch_pdl(kern, dim3(unsigned(grid)), dim3(256), size_t(smem), s, 1, x, ldx, vec, static_cast<const uint8_t*>(W), ldw,
              wide, static_cast<const uint32_t*>(Ws), fp8_rows_padded(N), C, ldc, int(M), int(N), int(K), epi);
@@ -1038,8 +1162,6 @@ void check_fp8_rows(const void* q, int64_t ldq, const void* scales, int64_t rows
        "data and scales must be 16-byte aligned");
 }
 
-bool vec_ok(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
-
 unsigned grid_for(int64_t blocks) {
   if (blocks >= (int64_t(1) << 31)) throw ApiError{LTX_ERR_UNSUPPORTED, "too many rows and columns for one launch"};
   return unsigned(blocks);
@@ -1056,9 +1178,8 @@ static void launch_quantize(const void* x, int64_t ldx, int64_t rows, int64_t co
                             int dtype, cudaStream_t s) {
   const int quads = int(fp8_quads(cols));
   const unsigned grid = grid_for((rows * quads + 7) / 8);
-  const int vec = vec_ok(x, ldx);
   auto run = [&](auto* xp, auto kern) {
-    launch_pdl(kern, dim3(grid), dim3(256), 0, s, 1, xp, ldx, rows, cols, quads, vec, static_cast<uint8_t*>(q), ldq,
+    launch_pdl(kern, dim3(grid), dim3(256), 0, s, 1, xp, ldx, rows, cols, quads, row_vec(xp, ldx), static_cast<uint8_t*>(q), ldq,
                static_cast<uint32_t*>(scales), fp8_rows_padded(rows));
   };
   if (dtype == LTX_F32)
@@ -1088,11 +1209,12 @@ extern "C" int ltx_dequantize_fp8(const void* q, int64_t ldq, const void* scales
   LTX_REQUIRE(ldx >= cols, "ldx must hold the columns");
   LTX_REQUIRE(reinterpret_cast<uintptr_t>(x) % (dtype == LTX_F32 ? 4 : 2) == 0, "x is not aligned to its type");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = grid_for((rows * ((cols + 7) / 8) + 255) / 256);
-  const int vec = vec_ok(x, ldx);
+  const int quads = int(fp8_quads(cols));
+  const unsigned grid = grid_for(((rows + kDequantRows - 1) / kDequantRows * quads + 7) / 8);
   auto run = [&](auto* xp, auto kern) {
     launch_pdl(kern, dim3(grid), dim3(256), 0, s, 1, static_cast<const uint8_t*>(q), ldq,
-               static_cast<const uint32_t*>(scales), fp8_rows_padded(rows), rows, cols, vec, xp, ldx);
+               static_cast<const uint32_t*>(scales), fp8_rows_padded(rows), rows, cols, quads, row_vec(xp, ldx), xp,
+               ldx);
   };
   if (dtype == LTX_F32)
     run(static_cast<float*>(x), dequantize_fp8_kernel<float>);
@@ -1133,9 +1255,38 @@ extern "C" int ltx_norm_modulate_fp8(const void* x, int64_t ldx, void* q, int64_
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto run = [&](auto* xp) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(xp)>>;
-    launch_pdl(norm_modulate_fp8_kernel<T>, dim3(unsigned(rows)), dim3(unsigned((D + 511) / 512 * 32)), 0, s, 1, xp,
-               ldx, rows_per_batch, D, norm_kind, eps, make_modvec<T>(mod, 0), make_modvec<T>(mod, 1),
-               static_cast<uint8_t*>(q), ldq, static_cast<uint32_t*>(scales), fp8_rows_padded(rows));
+    const ModVec<T> sh = make_modvec<T>(mod, 0), sc = make_modvec<T>(mod, 1);
+    const bool per_tok = (sh.on && sh.mod && sh.ldt != 0) || (sc.on && sc.mod && sc.ldt != 0);
+    const int wr = (D + kFp8Quad - 1) / kFp8Quad, groups = std::max(1, 8 / wr);
+    const int threads = 32 * wr * groups;  // <= 256 up to 4096 columns
+    const bool hoist = !per_tok && threads <= 512;
+    // as many CTAs as the SMs hold, each an even share of one sample's rows
+    const int64_t rpb = std::min(rows_per_batch, rows), samples = (rows + rows_per_batch - 1) / rows_per_batch;
+    const int64_t target = int64_t(num_sms()) * (threads <= 256 ? 3 * 256 / threads : threads <= 512 ? 1 : 2);
+    const int64_t per = std::min<int64_t>(rpb, std::max<int64_t>(groups, (rows + target - 1) / target));
+    const int64_t chunks = (rpb + per - 1) / per;
+    const unsigned grid = grid_for(samples * chunks);
+    auto go = [&](auto kern) {
+      launch_pdl(kern, dim3(grid), dim3(unsigned(threads)), 0, s, 1, xp, ldx, row_vec(xp, ldx), rows, rows_per_batch, D,
+                 wr, int(chunks), int(per), eps, sh, sc, static_cast<uint8_t*>(q), ldq, static_cast<uint32_t*>(scales),
+                 fp8_rows_padded(rows));
+    };
+    auto kind = [&](auto kc) {
+      constexpr int KIND = decltype(kc)::value;
+      if (hoist && threads <= 256)
+        go(norm_modulate_fp8_kernel<T, KIND, true, 256>);
+      else if (hoist)
+        go(norm_modulate_fp8_kernel<T, KIND, true, 512>);
+      else if (threads <= 256)
+        go(norm_modulate_fp8_kernel<T, KIND, false, 256>);
+      else
+        go(norm_modulate_fp8_kernel<T, KIND, false, 1024>);
+    };
+    switch (norm_kind) {
+      case LTX_NORM_RMS: kind(std::integral_constant<int, LTX_NORM_RMS>{}); break;
+      case LTX_NORM_LAYER: kind(std::integral_constant<int, LTX_NORM_LAYER>{}); break;
+      default: kind(std::integral_constant<int, LTX_NORM_NONE>{}); break;
+    }
   };
   if (dtype == LTX_F32)
     run(static_cast<const float*>(x));

@@ -30,12 +30,6 @@ LTX_DEVICE int64_t fp8_word(int64_t r, int64_t kq, int64_t rows_padded) {
   return kq * rows_padded + (r & ~int64_t(127)) + (r & 31) * 4 + ((r >> 5) & 3);
 }
 
-// |v| where it is finite, 0 where v is NaN or infinite (those take no part in a scale).
-LTX_DEVICE float fp8_abs_finite(float v) {
-  const float a = fabsf(v);
-  return a < __int_as_float(0x7f800000) ? a : 0.f;
-}
-
 // Scale code of a block whose largest finite magnitude is amax: code - 127 is the least
 // e >= -126 with amax <= 448 * 2^e = 1.75 * 2^(e + 8), read off amax = m * 2^E, 1 <= m < 2:
 // e = E - 8, one more where m > 1.75. A block of zeros has scale 1.
@@ -48,12 +42,17 @@ LTX_DEVICE int fp8_scale_code(float amax) {
 LTX_DEVICE float fp8_inv_scale(int code) { return __uint_as_float(uint32_t(254 - code) << 23); }
 LTX_DEVICE float fp8_scale(int code) { return __uint_as_float(uint32_t(code) << 23); }
 
-// Two values, already divided by their scale, to e4m3 (round to nearest even); lo in the
+// Four values, already divided by their scale, to e4m3 (round to nearest even), a in the
 // low byte. NaN gives the 8-bit NaN; the callers turn infinities into NaN first, since the
 // format has no infinity and the conversion would saturate them.
-LTX_DEVICE uint32_t fp8_pack2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+LTX_DEVICE uint32_t fp8_pack4(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}\n"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
   return r;
 }
 LTX_DEVICE void fp8_unpack2(uint32_t w, float& lo, float& hi) {
@@ -64,33 +63,47 @@ LTX_DEVICE void fp8_unpack2(uint32_t w, float& lo, float& hi) {
       : "r"(h));
 }
 
-// v / scale, NaN where v is infinite or NaN (v - v is 0 for finite v, NaN otherwise).
-LTX_DEVICE float fp8_scaled(float v, float inv) { return fmaf(v, inv, v - v); }
+// max(|a|, |b|, |c|), NaN if any of them is.
+LTX_DEVICE float max3_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Quantise the 16 consecutive columns this lane holds; the 8 lanes of an aligned group
 // share a block of 128 columns, the warp a quad of 512. Returns the block's scale code.
-LTX_DEVICE int fp8_quantize16(const float (&v)[16], uint4& out) {
-  float a = 0.f;
+// A warp without NaN and infinities (the maximum keeps both) takes neither the second
+// maximum, over finite values only, nor the replacement of infinities by NaN.
+LTX_DEVICE int fp8_quantize16(float (&v)[16], uint4& out) {
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) a = fmaxf(a, fp8_abs_finite(v[i]));
+  for (int i = 0; i < 16; i += 2) top = max3_abs_nan(top, v[i], v[i + 1]);
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const int code = fp8_scale_code(a);
+  for (int o = 1; o < 8; o <<= 1) top = max3_abs_nan(top, __shfl_xor_sync(0xffffffffu, top, o), 0.f);
+  const float inf = __int_as_float(0x7f800000);
+  if (__any_sync(0xffffffffu, !(top < inf))) {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (fabsf(v[i]) < inf)
+        top = fmaxf(top, fabsf(v[i]));
+      else
+        v[i] = __int_as_float(0x7fffffff);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  const int code = fp8_scale_code(top);
   const float inv = fp8_inv_scale(code);
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = fp8_pack2(fp8_scaled(v[4 * i], inv), fp8_scaled(v[4 * i + 1], inv)) |
-           (fp8_pack2(fp8_scaled(v[4 * i + 2], inv), fp8_scaled(v[4 * i + 3], inv)) << 16);
+  for (int i = 0; i < 4; ++i) w[i] = fp8_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
   out = make_uint4(w[0], w[1], w[2], w[3]);
   return code;
 }
-// The word of the warp's four blocks, from the codes of lanes 0, 8, 16, 24 (all lanes).
-LTX_DEVICE uint32_t fp8_quad_word(int code) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w |= uint32_t(__shfl_sync(0xffffffffu, code, 8 * j)) << (8 * j);
-  return w;
+// The warp's four scale bytes of a quad into its word, one from each group of 8 lanes.
+LTX_DEVICE void fp8_store_codes(uint32_t* word, int code) {
+  if ((lane_id() & 7) == 0) reinterpret_cast<uint8_t*>(word)[lane_id() >> 3] = uint8_t(code);
 }
 
 }  // namespace detail
