@@ -130,10 +130,9 @@ struct MaCfg {
   static constexpr int RING = TILE * 2 * (QBUF + STAGES);
   static constexpr int BIAS = STAGES * 128 * 4;
   static constexpr int LIST = MAX_TILES * 2;
-  static constexpr int SMEM = RING + BIAS + LIST + 512 + 1024;
+  static constexpr int SMEM = RING + BIAS + LIST + 768 + 1024;
   static constexpr int LD_PART = D + 4;           // floats per row of a split unit's partial
   static_assert(256 * LD_PART * 4 + 256 * 4 <= RING, "the partial reuses the operand ring");
-  static_assert((2 * QBUF + 4 * STAGES + 8) * 8 + STAGES * 16 + 8 <= 512, "barriers and descriptors");
   static constexpr uint32_t s_col(int i) { return uint32_t(128 * i); }
   static constexpr uint32_t p_col(int i) { return SEP_P ? uint32_t(256 + 64 * i) : uint32_t(128 * i); }
   static constexpr uint32_t o_col(int i) { return SEP_P ? uint32_t(384 + 64 * i) : uint32_t(256 + D * i); }
@@ -157,11 +156,28 @@ struct MaParams {
 // What a K / V stage holds: a key tile of a unit. FIRST / LAST of the unit's tiles; MARKED:
 // its scores need sbias; TWO: Q tile 1 of the unit has rows; END: no more tiles.
 struct MaTile {
-  int unit, tile, flags, pad;
+  int flags, unit, tile, pad;
 };
 enum : int { MA_FIRST = 1, MA_LAST = 2, MA_MARKED = 4, MA_TWO = 8, MA_END = 16 };
 
+// The same once per unit, for the softmax, whose tile loop then reads no descriptor (a wait
+// and a load per tile cost it 15 %): `tiles` of them (0: no more units), and which of the
+// first 64 are marked (of a longer unit's later tiles, the stage's descriptor says it).
+struct MaUnit {
+  int unit, tiles, flags, pad;
+  uint32_t marked[2];
+  uint32_t pad2[2];
+};
+constexpr int kMaUnits = 4;  // units the producer may be ahead
+
 LTX_DEVICE void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <int D>
+constexpr int ma_control_bytes() {
+  return (2 * MaCfg<D>::QBUF + 4 * MaCfg<D>::STAGES + 8 + 2 * kMaUnits) * 8 + MaCfg<D>::STAGES * int(sizeof(MaTile)) +
+         kMaUnits * int(sizeof(MaUnit)) + 8;
+}
+static_assert(ma_control_bytes<64>() <= 768 && ma_control_bytes<128>() <= 768, "barriers and descriptors");
 
 template <int D>
 __global__ void __launch_bounds__(384, 1)
@@ -186,8 +202,11 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* s_free = s_full + 2;             // [2] SEP_P only
   uint64_t* p_full = s_free + 2;             // [2]
   uint64_t* o_done = p_full + 2;             // [2]
-  MaTile* desc = reinterpret_cast<MaTile*>(o_done + 2);  // [S]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(desc + S);
+  uint64_t* u_full = o_done + 2;             // [kMaUnits] unit descriptor written
+  uint64_t* u_empty = u_full + kMaUnits;     // [kMaUnits] read by the eight softmax warps
+  MaTile* desc = reinterpret_cast<MaTile*>(u_empty + kMaUnits);  // [S]
+  MaUnit* units = reinterpret_cast<MaUnit*>(desc + S);           // [kMaUnits]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + kMaUnits);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = warp_id(), lane = lane_id();
@@ -207,6 +226,10 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(&s_free[i], 128);
       mbar_init(&p_full[i], 128);
       mbar_init(&o_done[i], 1);
+    }
+    for (int k = 0; k < kMaUnits; ++k) {
+      mbar_init(&u_full[k], 1);
+      mbar_init(&u_empty[k], 8);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -238,6 +261,7 @@ __global__ void __launch_bounds__(384, 1)
       tma_prefetch_desc(&tmV);
     }
     int b = -1, lo = 0, n = 0, g = 0, un = 0;
+    uint32_t marked[2] = {0, 0};  // of this CTA's first 64 tiles of the sample
     bool ok = true;
     for (int u = u0; ok && u < P.units; u += u_step) {
       const int nb = P.sample(u), h = P.head(u), q0 = P.q0(u);
@@ -269,6 +293,9 @@ __global__ void __launch_bounds__(384, 1)
         __syncwarp();
         lo = int(int64_t(count) * rank / P.split);
         n = int(int64_t(count) * (rank + 1) / P.split) - lo;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          marked[j] = __ballot_sync(0xffffffffu, 32 * j + lane < n && (list[lo + 32 * j + lane] & 0x8000));
       }
       if (n == 0) {
         if (P.split == 1) {  // no key: zero rows
@@ -281,8 +308,11 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (lane == 0) {
         const int k = un % Cfg::QBUF, col0 = h * D, two = q0 + 128 < P.Tq ? 1 : 0;
-        ok = mbar_wait(&q_empty[k], (uint32_t(un / Cfg::QBUF) & 1) ^ 1, abort_flag);
+        ok = mbar_wait(&u_empty[un % kMaUnits], (uint32_t(un / kMaUnits) & 1) ^ 1, abort_flag) &&
+             mbar_wait(&q_empty[k], (uint32_t(un / Cfg::QBUF) & 1) ^ 1, abort_flag);
         if (ok) {
+          units[un % kMaUnits] = MaUnit{u, n, two ? MA_TWO : 0, 0, {marked[0], marked[1]}, {0, 0}};
+          mbar_arrive(&u_full[un % kMaUnits]);
           mbar_arrive_expect_tx(&q_full[k], (1 + two) * Cfg::TILE);
           for (int i = 0; i <= two; ++i)
 #pragma unroll
@@ -295,8 +325,8 @@ __global__ void __launch_bounds__(384, 1)
           ok = mbar_wait(&kv_empty[s], (uint32_t(g / S) & 1) ^ 1, abort_flag);
           if (!ok) break;
           const int e = list[lo + t], tile = e & 0x7fff;
-          desc[s] = MaTile{u, tile, (t == 0 ? MA_FIRST : 0) | (t == n - 1 ? MA_LAST : 0) |
-                                       ((e & 0x8000) ? MA_MARKED : 0) | (two ? MA_TWO : 0), 0};
+          desc[s] = MaTile{(t == 0 ? MA_FIRST : 0) | (t == n - 1 ? MA_LAST : 0) | ((e & 0x8000) ? MA_MARKED : 0) |
+                               (two ? MA_TWO : 0), u, tile, 0};
           uint8_t* sk = sKV + 2 * s * Cfg::TILE;
           const int row = b * P.Tk + tile * 128;
           mbar_arrive_expect_tx(&k_full[s], Cfg::TILE);
@@ -311,8 +341,11 @@ __global__ void __launch_bounds__(384, 1)
       ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
       ++un;
     }
-    if (lane == 0 && ok && mbar_wait(&kv_empty[g % S], (uint32_t(g / S) & 1) ^ 1, abort_flag)) {
-      desc[g % S] = MaTile{0, 0, MA_END, 0};
+    if (lane == 0 && ok && mbar_wait(&u_empty[un % kMaUnits], (uint32_t(un / kMaUnits) & 1) ^ 1, abort_flag) &&
+        mbar_wait(&kv_empty[g % S], (uint32_t(g / S) & 1) ^ 1, abort_flag)) {
+      units[un % kMaUnits] = MaUnit{0, 0, 0, 0, {0, 0}, {0, 0}};
+      mbar_arrive(&u_full[un % kMaUnits]);
+      desc[g % S] = MaTile{MA_END, 0, 0, 0};
       mbar_arrive(&k_full[g % S]);
     }
   } else if (warp == 9 || warp == 10) {
@@ -470,21 +503,45 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t s_tmem = tmem + Cfg::s_col(qt) + lane_off;
     const uint32_t p_tmem = tmem + Cfg::p_col(qt) + lane_off;
     const uint32_t o_tmem = tmem + Cfg::o_col(qt) + lane_off;
-    for (int g = 0;; ++g) {
-      const int s = g % S;
-      if (!mbar_wait(&k_full[s], uint32_t(g / S) & 1, abort_flag)) break;
-      const int flags = desc[s].flags;
-      if (flags & MA_END) break;
-      if (!mbar_wait(&s_full[qt], uint32_t(g) & 1, abort_flag)) break;
-      if (qt == 1 && !(flags & MA_TWO)) {
-        if (Cfg::SEP_P) mbar_arrive(&s_free[qt]);
-        // one p_full phase ahead of the issuer at most, as below
-        if (g > 0 && !mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
-        mbar_arrive(&p_full[qt]);
+    bool ok = true;
+    int g = 0;
+    for (int un = 0; ok; ++un) {
+      if (!mbar_wait(&u_full[un % kMaUnits], uint32_t(un / kMaUnits) & 1, abort_flag)) break;
+      const MaUnit* ud = &units[un % kMaUnits];
+      const int unit = ud->unit, two = ud->flags & MA_TWO;
+      const int n = int(__reduce_max_sync(0xffffffffu, unsigned(ud->tiles)));  // warp-uniform
+      const uint32_t marked0 = ud->marked[0], marked1 = ud->marked[1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&u_empty[un % kMaUnits]);
+      if (n == 0) break;
+      if (qt == 1 && !two) {
+        for (int t = 0; t < n; ++t, ++g) {
+          // one p_full phase ahead of the issuer at most, as below
+          ok = mbar_wait(&s_full[qt], uint32_t(g) & 1, abort_flag) &&
+               (g == 0 || mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag));
+          if (!ok) break;
+          if (Cfg::SEP_P) mbar_arrive(&s_free[qt]);
+          mbar_arrive(&p_full[qt]);
+        }
         continue;
       }
-      const int unit = desc[s].unit;  // the stage may be refilled once P is handed over
-      const bool first = flags & MA_FIRST;
+      m_ref = -INFINITY;
+      l_run = 0.f;
+      for (int t = 0; t < n; ++t, ++g) {
+      const int s = g % S;
+      const bool first = t == 0;
+      if (!mbar_wait(&s_full[qt], uint32_t(g) & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+      bool marked = ((t < 32 ? marked0 : marked1) >> (t & 31)) & 1u;
+      if (t >= 64) {
+        if (!mbar_wait(&k_full[s], uint32_t(g / S) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        marked = desc[s].flags & MA_MARKED;
+      }
       tc_fence_after();
       float sv[128];
 #pragma unroll
@@ -494,21 +551,21 @@ __global__ void __launch_bounds__(384, 1)
         tc_fence_before();
         mbar_arrive(&s_free[qt]);
       }
-      float sc = P.scale_log2;
-      const bool marked = flags & MA_MARKED;
       if (marked) {
         // scores in log2 units with the mask added; a left-out key's is -inf whatever K held
-        if (!mbar_wait(&v_fix[s], uint32_t(g / S) & 1, abort_flag)) break;
+        if (!mbar_wait(&v_fix[s], uint32_t(g / S) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
         const float4* bias = reinterpret_cast<const float4*>(sbias + s * 128);
 #pragma unroll
         for (int e = 0; e < 128; e += 4) {
           const float4 bb = bias[e >> 2];
-          sv[e] = bb.x == -INFINITY ? -INFINITY : fmaf(sv[e], sc, bb.x);
-          sv[e + 1] = bb.y == -INFINITY ? -INFINITY : fmaf(sv[e + 1], sc, bb.y);
-          sv[e + 2] = bb.z == -INFINITY ? -INFINITY : fmaf(sv[e + 2], sc, bb.z);
-          sv[e + 3] = bb.w == -INFINITY ? -INFINITY : fmaf(sv[e + 3], sc, bb.w);
+          sv[e] = bb.x == -INFINITY ? -INFINITY : fmaf(sv[e], P.scale_log2, bb.x);
+          sv[e + 1] = bb.y == -INFINITY ? -INFINITY : fmaf(sv[e + 1], P.scale_log2, bb.y);
+          sv[e + 2] = bb.z == -INFINITY ? -INFINITY : fmaf(sv[e + 2], P.scale_log2, bb.z);
+          sv[e + 3] = bb.w == -INFINITY ? -INFINITY : fmaf(sv[e + 3], P.scale_log2, bb.w);
         }
-        sc = 1.f;
       }
       float m8[8];
 #pragma unroll
@@ -518,11 +575,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
       const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-      const float m_cand = mx * sc;
-      if (first) {
-        m_ref = -INFINITY;
-        l_run = 0.f;
-      }
+      const float m_cand = marked ? mx : mx * P.scale_log2;
       const bool need = first || (m_cand > m_ref + 8.f);
       float alpha = 1.f;
       if (need) {
@@ -531,31 +584,42 @@ __global__ void __launch_bounds__(384, 1)
         m_ref = m_new;
       }
       const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;  // a row of -inf so far: weights 0
-      const uint64_t sc2 = f2_pack(sc, sc);
       const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
       uint64_t rs2[4] = {0, 0, 0, 0};
       uint32_t pk[64];
+      auto weights = [&](auto plain) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x0, x1, p0, p1;
-          f2_unpack(f2_fma(f2_pack(sv[c * 32 + e], sv[c * 32 + e + 1]), sc2, nm2), x0, x1);
-          if (!marked && ((kFaPolyPairs >> (c * 16 + (e >> 1))) & 1u)) {
-            ex2_poly2(x0, x1, p0, p1);
-          } else {
-            p0 = ex2_approx(x0);
-            p1 = ex2_approx(x1);
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1, p0, p1;
+            const uint64_t s2 = f2_pack(sv[c * 32 + e], sv[c * 32 + e + 1]);
+            f2_unpack(decltype(plain)::value ? f2_fma(s2, f2_pack(P.scale_log2, P.scale_log2), nm2) : f2_add(s2, nm2), x0,
+                      x1);
+            if (decltype(plain)::value && ((kFaPolyPairs >> (c * 16 + (e >> 1))) & 1u)) {
+              ex2_poly2(x0, x1, p0, p1);
+            } else {
+              p0 = ex2_approx(x0);
+              p1 = ex2_approx(x1);
+            }
+            rs2[(e >> 1) & 3] = f2_add(rs2[(e >> 1) & 3], f2_pack(p0, p1));
+            pk[c * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
           }
-          rs2[(e >> 1) & 3] = f2_add(rs2[(e >> 1) & 3], f2_pack(p0, p1));
-          pk[c * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
+          if constexpr (!Cfg::SEP_P)
+            tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
         }
-        if constexpr (!Cfg::SEP_P) tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
-      }
+      };
+      if (marked)
+        weights(std::false_type{});
+      else
+        weights(std::true_type{});
       if constexpr (Cfg::SEP_P) {
         // P_i V_{g-1} has read P_i, and the issuer has seen p_full of tile g - 1
         if (g > 0) {
-          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
+          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
         }
 #pragma unroll
@@ -566,7 +630,10 @@ __global__ void __launch_bounds__(384, 1)
       f2_unpack(f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3])), r0, r1);
       if (!first && __any_sync(0xffffffffu, need)) {
         if (!Cfg::SEP_P) {
-          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
+          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
         }
 #pragma unroll
@@ -583,13 +650,13 @@ __global__ void __launch_bounds__(384, 1)
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[qt]);
-      if (!(flags & MA_LAST)) continue;
+      }
       // ------------------------- the unit's output rows -------------------------
-      if (!mbar_wait(&o_done[qt], uint32_t(g) & 1, abort_flag)) break;
+      if (!ok || !mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
       tc_fence_after();
       if (P.split > 1) {
         have = true;
-        continue;  // the END descriptor follows
+        break;  // the only unit
       }
       const int b = P.sample(unit), h = P.head(unit);
       const int qi = P.q0(unit) + qt * 128 + row;
