@@ -503,6 +503,108 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t s_tmem = tmem + Cfg::s_col(qt) + lane_off;
     const uint32_t p_tmem = tmem + Cfg::p_col(qt) + lane_off;
     const uint32_t o_tmem = tmem + Cfg::o_col(qt) + lane_off;
+    // Softmax of tile g (`first` of its unit) from S to P. Plain and marked tiles are separate
+    // code: the plain one is that of attention.cu, without the mask's registers.
+    auto tile = [&](auto marked_c, int g, bool first) {
+      constexpr bool MARKED = decltype(marked_c)::value;
+      const int s = g % S;
+      if (!mbar_wait(&s_full[qt], uint32_t(g) & 1, abort_flag)) return false;
+      tc_fence_after();
+      uint32_t su[128];
+      tmem_read128(s_tmem, su);
+      float sv[128];
+#pragma unroll
+      for (int e = 0; e < 128; ++e) sv[e] = __uint_as_float(su[e]);
+      if constexpr (Cfg::SEP_P) {
+        tc_fence_before();
+        mbar_arrive(&s_free[qt]);
+      }
+      if constexpr (MARKED) {
+        // scores in log2 units with the mask added; a left-out key's is -inf whatever K held
+        if (!mbar_wait(&v_fix[s], uint32_t(g / S) & 1, abort_flag)) return false;
+        const float4* bias = reinterpret_cast<const float4*>(sbias + s * 128);
+#pragma unroll
+        for (int e = 0; e < 128; e += 4) {
+          const float4 bb = bias[e >> 2];
+          sv[e] = bb.x == -INFINITY ? -INFINITY : fmaf(sv[e], P.scale_log2, bb.x);
+          sv[e + 1] = bb.y == -INFINITY ? -INFINITY : fmaf(sv[e + 1], P.scale_log2, bb.y);
+          sv[e + 2] = bb.z == -INFINITY ? -INFINITY : fmaf(sv[e + 2], P.scale_log2, bb.z);
+          sv[e + 3] = bb.w == -INFINITY ? -INFINITY : fmaf(sv[e + 3], P.scale_log2, bb.w);
+        }
+      }
+      float m8[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m8[e] = sv[e];
+#pragma unroll
+      for (int e = 8; e < 120; e += 16)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m8[j] = fmaxf(m8[j], sv[120 + j]);
+      const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+      const float m_cand = MARKED ? mx : mx * P.scale_log2;
+      const bool need = first || (m_cand > m_ref + 8.f);
+      float alpha = 1.f;
+      if (need) {
+        const float m_new = fmaxf(m_ref, m_cand);
+        alpha = first || m_new == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
+        m_ref = m_new;
+      }
+      const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;  // a row of -inf so far: weights 0
+      const uint64_t sc2 = f2_pack(P.scale_log2, P.scale_log2);
+      const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
+      uint64_t rs2[4] = {0, 0, 0, 0};
+      uint32_t pk[64];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float x0, x1, p0, p1;
+          const uint64_t s2 = f2_pack(sv[c * 32 + e], sv[c * 32 + e + 1]);
+          f2_unpack(MARKED ? f2_add(s2, nm2) : f2_fma(s2, sc2, nm2), x0, x1);
+          if (!MARKED && ((kFaPolyPairs >> (c * 16 + (e >> 1))) & 1u)) {
+            ex2_poly2(x0, x1, p0, p1);
+          } else {
+            p0 = ex2_approx(x0);
+            p1 = ex2_approx(x1);
+          }
+          rs2[(e >> 1) & 3] = f2_add(rs2[(e >> 1) & 3], f2_pack(p0, p1));
+          pk[c * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
+        }
+        if constexpr (!Cfg::SEP_P) tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
+      }
+      if constexpr (Cfg::SEP_P) {
+        // P_i V_{g-1} has read P_i, and the issuer has seen p_full of tile g - 1
+        if (g > 0) {
+          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) return false;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
+      }
+      float r0, r1;
+      f2_unpack(f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3])), r0, r1);
+      if (!first && __any_sync(0xffffffffu, need)) {
+        if (!Cfg::SEP_P) {
+          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) return false;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t rr[32];
+          tmem_read32(o_tmem + uint32_t(c0), rr);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) rr[e] = __float_as_uint(__uint_as_float(rr[e]) * alpha);
+          tmem_st32(o_tmem + uint32_t(c0), rr);
+        }
+      }
+      l_run = l_run * alpha + (r0 + r1);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[qt]);
+      return true;
+    };
     bool ok = true;
     int g = 0;
     for (int un = 0; ok; ++un) {
@@ -528,128 +630,14 @@ __global__ void __launch_bounds__(384, 1)
       m_ref = -INFINITY;
       l_run = 0.f;
       for (int t = 0; t < n; ++t, ++g) {
-      const int s = g % S;
-      const bool first = t == 0;
-      if (!mbar_wait(&s_full[qt], uint32_t(g) & 1, abort_flag)) {
-        ok = false;
-        break;
-      }
-      bool marked = ((t < 32 ? marked0 : marked1) >> (t & 31)) & 1u;
-      if (t >= 64) {
-        if (!mbar_wait(&k_full[s], uint32_t(g / S) & 1, abort_flag)) {
-          ok = false;
-          break;
+        bool marked = ((t < 32 ? marked0 : marked1) >> (t & 31)) & 1u;
+        if (t >= 64) {
+          ok = mbar_wait(&k_full[g % S], uint32_t(g / S) & 1, abort_flag);
+          if (!ok) break;
+          marked = desc[g % S].flags & MA_MARKED;
         }
-        marked = desc[s].flags & MA_MARKED;
-      }
-      tc_fence_after();
-      float sv[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + uint32_t(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&sv[c * 32]));
-      tmem_wait_ld();
-      if constexpr (Cfg::SEP_P) {
-        tc_fence_before();
-        mbar_arrive(&s_free[qt]);
-      }
-      if (marked) {
-        // scores in log2 units with the mask added; a left-out key's is -inf whatever K held
-        if (!mbar_wait(&v_fix[s], uint32_t(g / S) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        const float4* bias = reinterpret_cast<const float4*>(sbias + s * 128);
-#pragma unroll
-        for (int e = 0; e < 128; e += 4) {
-          const float4 bb = bias[e >> 2];
-          sv[e] = bb.x == -INFINITY ? -INFINITY : fmaf(sv[e], P.scale_log2, bb.x);
-          sv[e + 1] = bb.y == -INFINITY ? -INFINITY : fmaf(sv[e + 1], P.scale_log2, bb.y);
-          sv[e + 2] = bb.z == -INFINITY ? -INFINITY : fmaf(sv[e + 2], P.scale_log2, bb.z);
-          sv[e + 3] = bb.w == -INFINITY ? -INFINITY : fmaf(sv[e + 3], P.scale_log2, bb.w);
-        }
-      }
-      float m8[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m8[e] = sv[e];
-#pragma unroll
-      for (int e = 8; e < 128; e += 16)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
-      const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-      const float m_cand = marked ? mx : mx * P.scale_log2;
-      const bool need = first || (m_cand > m_ref + 8.f);
-      float alpha = 1.f;
-      if (need) {
-        const float m_new = fmaxf(m_ref, m_cand);
-        alpha = first || m_new == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
-        m_ref = m_new;
-      }
-      const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;  // a row of -inf so far: weights 0
-      const uint64_t nm2 = f2_pack(-m_sub, -m_sub);
-      uint64_t rs2[4] = {0, 0, 0, 0};
-      uint32_t pk[64];
-      auto weights = [&](auto plain) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float x0, x1, p0, p1;
-            const uint64_t s2 = f2_pack(sv[c * 32 + e], sv[c * 32 + e + 1]);
-            f2_unpack(decltype(plain)::value ? f2_fma(s2, f2_pack(P.scale_log2, P.scale_log2), nm2) : f2_add(s2, nm2), x0,
-                      x1);
-            if (decltype(plain)::value && ((kFaPolyPairs >> (c * 16 + (e >> 1))) & 1u)) {
-              ex2_poly2(x0, x1, p0, p1);
-            } else {
-              p0 = ex2_approx(x0);
-              p1 = ex2_approx(x1);
-            }
-            rs2[(e >> 1) & 3] = f2_add(rs2[(e >> 1) & 3], f2_pack(p0, p1));
-            pk[c * 16 + (e >> 1)] = pack_bf16x2(p0, p1);
-          }
-          if constexpr (!Cfg::SEP_P)
-            tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
-        }
-      };
-      if (marked)
-        weights(std::false_type{});
-      else
-        weights(std::true_type{});
-      if constexpr (Cfg::SEP_P) {
-        // P_i V_{g-1} has read P_i, and the issuer has seen p_full of tile g - 1
-        if (g > 0) {
-          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_st16(p_tmem + uint32_t(c * 16), *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
-      }
-      float r0, r1;
-      f2_unpack(f2_add(f2_add(rs2[0], rs2[1]), f2_add(rs2[2], rs2[3])), r0, r1);
-      if (!first && __any_sync(0xffffffffu, need)) {
-        if (!Cfg::SEP_P) {
-          if (!mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-        }
-#pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t rr[32];
-          tmem_ld32(o_tmem + uint32_t(c0), rr);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) rr[e] = __float_as_uint(__uint_as_float(rr[e]) * alpha);
-          tmem_st32(o_tmem + uint32_t(c0), rr);
-        }
-      }
-      l_run = l_run * alpha + (r0 + r1);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[qt]);
+        ok = marked ? tile(std::true_type{}, g, t == 0) : tile(std::false_type{}, g, t == 0);
+        if (!ok) break;
       }
       // ------------------------- the unit's output rows -------------------------
       if (!ok || !mbar_wait(&o_done[qt], uint32_t(g - 1) & 1, abort_flag)) break;
@@ -668,8 +656,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t rr[32];
-        tmem_ld32(o_tmem + uint32_t(c0), rr);
-        tmem_wait_ld();
+        tmem_read32(o_tmem + uint32_t(c0), rr);
         if (live) {
 #pragma unroll
           for (int e8 = 0; e8 < 32; e8 += 8) {
@@ -694,8 +681,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t rr[32];
-          tmem_ld32(o_tmem + uint32_t(c0), rr);
-          tmem_wait_ld();
+          tmem_read32(o_tmem + uint32_t(c0), rr);
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             *reinterpret_cast<float4*>(part + r * Cfg::LD_PART + c0 + e) =

@@ -627,8 +627,7 @@ __global__ void __launch_bounds__(192, 2)
 #pragma unroll 1
       for (int c0 = 0; c0 < 128 && n0 + c0 < N; c0 += 32) {
         uint32_t rr[32];
-        tmem_ld32(tquad + uint32_t(c0), rr);
-        tmem_wait_ld();
+        tmem_read32(tquad + uint32_t(c0), rr);
         if (!live) continue;
         if (staged) {
           // every MMA of this CTA has read its operands: the ring is free
@@ -844,8 +843,7 @@ __global__ void __launch_bounds__(320, 1)
       for (int j = 0; j < 4; ++j) {
         const int c0 = half * 128 + (acc ? j : 3 - j) * 32;
         uint32_t rr[32];
-        tmem_ld32(tbase + uint32_t(c0), rr);
-        tmem_wait_ld();
+        tmem_read32(tbase + uint32_t(c0), rr);
         if (j == 0 && shares) {
           tc_fence_before();
           __syncwarp();
