@@ -21,6 +21,11 @@ through _native (no cuBLAS, no cuDNN, no torch element-wise math on the path):
 Activations are (B*T, D) row-major buffers in HBM; the residual stream is updated in
 place by the GEMM epilogues.
 
+LTXModel.quantize_fp8 moves the blocks' products to 8-bit rows (e4m3 with a power-of-two
+scale per 128 columns): the norms write them, the tensor cores multiply them with their
+scales, and the residual stream, attention and adaLN stay in the model's type. A text
+context that is padded carries its mask in Modality.context_mask.
+
 Guidance: cfg_denoise_step is the fused CFG-only step (B=2, X0 + CFG + Euler in the
 proj_out epilogue). guided_denoise_step / run_dit run the reference's full guidance: one
 B=4 forward over [cond, uncond, STG-perturbed, modality-isolated] (perturbed
@@ -38,7 +43,8 @@ from dataclasses import dataclass, replace
 import torch
 
 import _native as nat
-from ltx_nn import AdaLayerNormSingle, Attention, FeedForward, RopeTables, rope_tables
+from ltx_nn import (AdaLayerNormSingle, Attention, FeedForward, RopeTables, key_mask, norm_into, project,
+                    rope_tables)
 
 DEVICE = torch.device("cuda")
 
@@ -141,6 +147,7 @@ class Modality:
     context: torch.Tensor  # (B, S, cross_dim) text encoding
     keyframes_mask: torch.Tensor | None = None  # (B, T, 1)
     enabled: bool = True
+    context_mask: torch.Tensor | None = None  # (B, S) over context: bool (True: a token) or additive
 
 
 @dataclass
@@ -166,6 +173,7 @@ class _Stream:
     cross_gate: torch.Tensor | None  # (B, D)
     enabled: bool
     context_src: torch.Tensor | None = None  # the caller's context tensor (cache identity)
+    context_mask: torch.Tensor | None = None  # (B or 1, S) key mask of the text cross-attention
 
     def mod(self, table: torch.Tensor, tmod: torch.Tensor, shift: int | None, scale: int | None,
             n_total: int | None = None, ld_tok: int | None = None) -> nat.Modulation:
@@ -243,6 +251,25 @@ class LTXModel(torch.nn.Module):
         self._kv_cache: dict = {}
         self._cat_cache = None
         self._sp = None  # ltx_parallel.SequenceParallel when the video tokens are sharded
+
+    def quantize_fp8(self) -> "LTXModel":
+        """Run the blocks' projections and feed-forwards on 8-bit rows from now on: every
+        weight of theirs gets an 8-bit form (ltx_nn.quantize_fp8, one byte per weight beside
+        the parameter), every norm in front of a product writes 8-bit rows, other operands
+        are quantised by the product's call. The projection of a text context that is cached
+        over the denoise steps, the adaLN layers, the patchify and output projections and
+        all of attention stay in the model's type. Call it again after loading other
+        weights. NativeStep keeps running the parameters as they are."""
+        for blk in self.blocks:
+            for attn in (blk.attn1, blk.audio_attn1):
+                attn.quantize_fp8(("self",))
+            for attn in (blk.attn2, blk.audio_attn2):
+                attn.quantize_fp8(("q", "kv") if self.cfg.cross_attention_adaln else ("q",))
+            for attn in (blk.audio_to_video_attn, blk.video_to_audio_attn):
+                attn.quantize_fp8(("q", "kv"))
+            blk.ff.quantize_fp8()
+            blk.audio_ff.quantize_fp8()
+        return self
 
     # ------------------------------------------------------------------ preparation
     def _rope(self, positions: torch.Tensor, dim: int, dtype: torch.dtype, max_pos: list, heads: int) -> RopeTables:
@@ -345,7 +372,8 @@ class LTXModel(torch.nn.Module):
             factor = cfg.av_ca_timestep_scale_multiplier / cfg.timestep_scale_multiplier
             cross_gate, _ = g_mod(cross.sigma.to(torch.float32).reshape(-1).contiguous(), dtype, scale * factor)
         return _Stream(stream, b, t, dim, heads, hd, x, tmod, 0 if t_sample is not None else 1, emb, prompt,
-                       context, s_len, pe, cross_pe, cross_ss, cross_gate, m.enabled, context_src=m.context)
+                       context, s_len, pe, cross_pe, cross_ss, cross_gate, m.enabled, context_src=m.context,
+                       context_mask=key_mask(m.context_mask, b, s_len) if m.context_mask is not None else None)
 
     # ------------------------------------------------------------------ block pieces
     def _self_and_text(self, blk: Block, st: _Stream, h: torch.Tensor, keep_self: list | None = None):
@@ -361,17 +389,16 @@ class LTXModel(torch.nn.Module):
         inner = attn1.heads * attn1.dim_head
         gated = cfg.gated_attention
         # self-attention
-        nat.norm_modulate(st.x, h, st.T, nat.LTX_NORM_RMS, eps, st.mod(table, st.tmod, 0, 1))
+        hs = norm_into(st.x, h, st.T, nat.LTX_NORM_RMS, eps, st.mod(table, st.tmod, 0, 1), "self" in attn1.fp8)
         perturbed = [b for b, k in enumerate(keep_self) if k == 0] if keep_self is not None else []
         if self._sp is not None and not a and not perturbed and self._sp.fused_for(attn1, st):
             # sequence-parallel over peer memory: q/k normalisation fused into the exchange
-            qkv = attn1.project_qkv(h, st.T, st.pe, normalize=False)
+            qkv = attn1.project_qkv(hs, st.T, st.pe, normalize=False)
             o = self._sp.self_attention_fused(attn1, qkv, st)
-            nat.linear(o, attn1.to_out.weight, st.x,
-                       nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn1.to_out.bias, residual=st.x,
-                                    gate=st.mod(table, st.tmod, None, 2), rows_per_batch=st.T))
+            attn1.project_out(o, st.x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn1.to_out.bias, residual=st.x,
+                                                    gate=st.mod(table, st.tmod, None, 2), rows_per_batch=st.T))
             return self._text_cross(blk, st, h, attn2, table, d, eps, rows, inner, gated)
-        qkv = attn1.project_qkv(h, st.T, st.pe)
+        qkv = attn1.project_qkv(hs, st.T, st.pe)
         v_cols = qkv[:, 2 * inner:3 * inner]
         g_cols = qkv[:, 3 * inner:3 * inner + attn1.heads] if gated else None
         if self._sp is not None and not a:
@@ -389,9 +416,8 @@ class LTXModel(torch.nn.Module):
                 r0, r1 = b * st.T, (b + 1) * st.T
                 nat.value_gate(v_cols[r0:r1], g_cols[r0:r1] if gated else None, o[r0:r1], attn1.heads,
                                attn1.dim_head)
-        nat.linear(o, attn1.to_out.weight, st.x,
-                   nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn1.to_out.bias, residual=st.x,
-                                gate=st.mod(table, st.tmod, None, 2), rows_per_batch=st.T))
+        attn1.project_out(o, st.x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn1.to_out.bias, residual=st.x,
+                                                gate=st.mod(table, st.tmod, None, 2), rows_per_batch=st.T))
         self._text_cross(blk, st, h, attn2, table, d, eps, rows, inner, gated)
 
     def _text_cross(self, blk: Block, st: _Stream, h: torch.Tensor, attn2, table, d: int, eps: float, rows: int,
@@ -400,47 +426,41 @@ class LTXModel(torch.nn.Module):
         cfg = self.cfg
         a = st.name == "audio"
         # text cross-attention
-        if cfg.cross_attention_adaln:
-            nat.norm_modulate(st.x, h, st.T, nat.LTX_NORM_RMS, eps, st.mod(table, st.tmod, 6, 7))
-        else:
-            nat.norm_modulate(st.x, h, st.T, nat.LTX_NORM_RMS, eps, None)
+        hq = norm_into(st.x, h, st.T, nat.LTX_NORM_RMS, eps,
+                       st.mod(table, st.tmod, 6, 7) if cfg.cross_attention_adaln else None, "q" in attn2.fp8)
         wq, bq = attn2.packed_q()
         qg = torch.empty(rows, wq.shape[0], device=h.device, dtype=h.dtype)
-        nat.linear(h, wq, qg, nat.epilogue(bias=bq))
+        project(hq, wq, attn2.fp8.get("q"), qg, nat.epilogue(bias=bq))
         attn2._norm_rope(qg[:, :inner], st.T, attn2.q_norm.weight, None)
         ctx = st.context
         if cfg.cross_attention_adaln:
             psst = blk.audio_prompt_scale_shift_table if a else blk.prompt_scale_shift_table
             if ctx.shape[1] != d:
                 raise ValueError("cross-adaLN needs the text context width to equal the hidden size")
-            enc = torch.empty_like(ctx)
-            nat.norm_modulate(ctx, enc, st.S, nat.LTX_NORM_NONE, eps,
-                              nat.modulation(psst, st.prompt_mod, shift=(0, 0), scale=(d, d),
-                                             mod_ld_batch=st.prompt_mod.shape[-1]))
+            fp8 = "kv" in attn2.fp8
+            enc = norm_into(ctx, ctx if fp8 else torch.empty_like(ctx), st.S, nat.LTX_NORM_NONE, eps,
+                            nat.modulation(psst, st.prompt_mod, shift=(0, 0), scale=(d, d),
+                                           mod_ld_batch=st.prompt_mod.shape[-1]), fp8)
             wkv, bkv = attn2.packed_kv()
-            kv = torch.empty(enc.shape[0], wkv.shape[0], device=h.device, dtype=h.dtype)
-            nat.linear(enc, wkv, kv, nat.epilogue(bias=bkv))
+            kv = torch.empty(ctx.shape[0], wkv.shape[0], device=h.device, dtype=h.dtype)
+            project(enc, wkv, attn2.fp8.get("kv"), kv, nat.epilogue(bias=bkv))
             attn2._norm_rope(kv[:, :inner], st.S, attn2.k_norm.weight, None)
         else:
             kv = self._text_kv(attn2, ctx, st.S, st.context_src if st.context_src is not None else ctx)
         o = attn2.attend(qg[:, :inner], kv[:, :inner], kv[:, inner:2 * inner], qg[:, inner:] if gated else None,
-                         st.B, st.T, st.S)
+                         st.B, st.T, st.S, st.context_mask)
         gate = st.mod(table, st.tmod, None, 8) if cfg.cross_attention_adaln else None
-        nat.linear(o, attn2.to_out.weight, st.x,
-                   nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn2.to_out.bias, residual=st.x, gate=gate,
-                                rows_per_batch=st.T))
+        attn2.project_out(o, st.x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn2.to_out.bias, residual=st.x, gate=gate,
+                                                rows_per_batch=st.T))
 
     def _ffn(self, blk: Block, st: _Stream, h: torch.Tensor):
         """Feed-forward with adaLN (ltx_dit.py:309-314)."""
         a = st.name == "audio"
         ff = blk.audio_ff if a else blk.ff
         table = blk.audio_scale_shift_table if a else blk.scale_shift_table
-        nat.norm_modulate(st.x, h, st.T, nat.LTX_NORM_RMS, self.cfg.norm_eps, st.mod(table, st.tmod, 3, 4))
-        f = torch.empty(st.B * st.T, ff.proj_in.out_features, device=h.device, dtype=h.dtype)
-        nat.linear(h, ff.proj_in.weight, f, nat.epilogue(nat.EPI_GELU_TANH, bias=ff.proj_in.bias))
-        nat.linear(f, ff.proj_out.weight, st.x,
-                   nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=ff.proj_out.bias, residual=st.x,
-                                gate=st.mod(table, st.tmod, None, 5), rows_per_batch=st.T))
+        h = norm_into(st.x, h, st.T, nat.LTX_NORM_RMS, self.cfg.norm_eps, st.mod(table, st.tmod, 3, 4), "in" in ff.fp8)
+        ff.run(h, st.x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=ff.proj_out.bias, residual=st.x,
+                                     gate=st.mod(table, st.tmod, None, 5), rows_per_batch=st.T))
 
     def _av_cross(self, blk: Block, vs: _Stream, as_: _Stream, run_a2v: bool, run_v2a: bool,
                   keep_a2v: list | None = None, keep_v2a: list | None = None):
@@ -451,12 +471,13 @@ class LTXModel(torch.nn.Module):
         eps = cfg.norm_eps
         tv, ta = blk.scale_shift_table_a2v_ca_video, blk.scale_shift_table_a2v_ca_audio
 
+        fp8 = "q" in blk.audio_to_video_attn.fp8
+
         def normed(st, table, rows_sl):
-            out = torch.empty_like(st.x)
             # get_av_ca_ada_values returns (scale, shift) = table rows (r0, r0 + 1)
             r0 = rows_sl
-            nat.norm_modulate(st.x, out, st.T, nat.LTX_NORM_RMS, eps, st.mod(table, st.cross_ss, r0 + 1, r0))
-            return out
+            return norm_into(st.x, st.x if fp8 else torch.empty_like(st.x), st.T, nat.LTX_NORM_RMS, eps,
+                             st.mod(table, st.cross_ss, r0 + 1, r0), fp8)
 
         def gate_of(st, table):
             d = table.shape[-1]
@@ -480,12 +501,12 @@ class LTXModel(torch.nn.Module):
         inner = attn.heads * attn.dim_head
         gated = self.cfg.gated_attention
         wq, bq = attn.packed_q()
-        qg = torch.empty(q_in.shape[0], wq.shape[0], device=q_in.device, dtype=q_in.dtype)
-        nat.linear(q_in, wq, qg, nat.epilogue(bias=bq))
+        qg = torch.empty(q_in.shape[0], wq.shape[0], device=wq.device, dtype=wq.dtype)
+        project(q_in, wq, attn.fp8.get("q"), qg, nat.epilogue(bias=bq))
         attn._norm_rope(qg[:, :inner], q_st.T, attn.q_norm.weight, q_pe)
         wkv, bkv = attn.packed_kv()
-        kv = torch.empty(kv_in.shape[0], wkv.shape[0], device=q_in.device, dtype=q_in.dtype)
-        nat.linear(kv_in, wkv, kv, nat.epilogue(bias=bkv))
+        kv = torch.empty(kv_in.shape[0], wkv.shape[0], device=wq.device, dtype=wq.dtype)
+        project(kv_in, wkv, attn.fp8.get("kv"), kv, nat.epilogue(bias=bkv))
         attn._norm_rope(kv[:, :inner], kv_st.T, attn.k_norm.weight, k_pe)
         if self._sp is not None and kv_st.name == "video":
             # video-to-audio under sequence parallelism: the video keys are sharded over
@@ -508,9 +529,9 @@ class LTXModel(torch.nn.Module):
         t = out_st.T
         for b0, b1 in runs:
             x = out_st.x[b0 * t:b1 * t]
-            nat.linear(o[b0 * t:b1 * t], attn.to_out.weight, x,
-                       nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn.to_out.bias, residual=x, gate=gate_at(b0),
-                                    rows_per_batch=t))
+            attn.project_out(o[b0 * t:b1 * t], x,
+                             nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn.to_out.bias, residual=x, gate=gate_at(b0),
+                                          rows_per_batch=t))
 
     # ------------------------------------------------------------------ forward
     def _keep_masks(self, perturbations, batch: int):
@@ -777,14 +798,30 @@ def _sigma_pair(sigmas: torch.Tensor, idx: int) -> tuple[float, float]:
     return float(s[idx]), float(s[idx + 1])
 
 
+def _cat_masks(masks: list[torch.Tensor | None], tokens: int) -> torch.Tensor | None:
+    """The (B, S) context mask of a guidance batch from its passes' (1, S) masks; a pass
+    without one keeps every token. None when no pass has a mask."""
+    given = next((m for m in masks if m is not None), None)
+    if given is None:
+        return None
+    full = torch.ones if given.dtype == torch.bool else torch.zeros
+    rows = [m.reshape(1, tokens) if m is not None else full(1, tokens, dtype=given.dtype, device=given.device)
+            for m in masks]
+    if any(r.dtype != given.dtype for r in rows):
+        raise TypeError("the context masks of a guidance batch must have one type")
+    return torch.cat(rows, dim=0)
+
+
 @torch.inference_mode()
 def cfg_denoise_step(model: LTXModel, latent: torch.Tensor, positions: torch.Tensor, context_pos: torch.Tensor,
                      context_neg: torch.Tensor, sigmas: torch.Tensor, idx: int, cfg_scale: float,
-                     keyframes_mask: torch.Tensor | None = None, fused_head: bool = True):
+                     keyframes_mask: torch.Tensor | None = None, fused_head: bool = True,
+                     context_mask_pos: torch.Tensor | None = None, context_mask_neg: torch.Tensor | None = None):
     """One CFG denoise step of the video stream (B = 2 [cond, uncond] forward, X0,
     guide, Euler; ltx_dit.py:565-606 with CFG-only guidance).
 
-    latent (1, T, C), positions (1, 3, T, 2), contexts (1, S, Cctx). Returns
+    latent (1, T, C), positions (1, 3, T, 2), contexts (1, S, Cctx), context masks (1, S) (a
+    context without one has no padding). Returns
     (velocity (2, T, C), denoised (1, T, C), next latent (1, T, C)). The X0 + CFG + Euler
     update runs in the proj_out GEMM epilogue (bf16) or right after it (fp32)."""
     dtype = model.proj_out.weight.dtype
@@ -796,7 +833,8 @@ def cfg_denoise_step(model: LTXModel, latent: torch.Tensor, positions: torch.Ten
     lat = latent.to(dtype)
     video = Modality(latent=lat.expand(2, -1, -1), sigma=sig, timesteps=ts, positions=positions.expand(2, -1, -1, -1),
                      context=model.cached_cat(context_pos, context_neg, dtype),
-                     keyframes_mask=keyframes_mask.expand(2, -1, -1) if keyframes_mask is not None else None)
+                     keyframes_mask=keyframes_mask.expand(2, -1, -1) if keyframes_mask is not None else None,
+                     context_mask=_cat_masks([context_mask_pos, context_mask_neg], context_pos.shape[1]))
     va, _ = model.prepare(video, None, uniform_timesteps=True)
     model.run_blocks(va, None)
     h = model.head_hidden(va)
@@ -997,7 +1035,9 @@ def guided_denoise_step(model: LTXModel, video_state: LatentState, audio_state: 
                         cfg: DiTConfig):
     """One transformer call with the B=4 guidance passes [cond, uncond, ptb (STG), mod
     (A<->V isolated)] -> blended x0 per modality (ltx_dit.py:565-599): the perturbation
-    keep-mask of build_perturbation_config, X0 per pass, guide() with rescale."""
+    keep-mask of build_perturbation_config, X0 per pass, guide() with rescale. `contexts`
+    may hold the (1, S) masks of padded contexts: v_pos_mask, v_neg_mask, a_pos_mask,
+    a_neg_mask."""
     passes = ["cond", "uncond", "ptb", "mod"]
     n = len(passes)
     sigma = sigma.reshape(()).to(torch.float32)
@@ -1010,14 +1050,19 @@ def guided_denoise_step(model: LTXModel, video_state: LatentState, audio_state: 
                      timesteps=video_state.denoise_mask.repeat(n, 1, 1) * sigma_b.view(n, 1, 1),
                      positions=video_state.positions.repeat(n, 1, 1, 1), context=v_ctx,
                      keyframes_mask=video_state.keyframes_mask.repeat(n, 1, 1)
-                     if video_state.keyframes_mask is not None else None)
+                     if video_state.keyframes_mask is not None else None,
+                     context_mask=_cat_masks([contexts.get("v_pos_mask"), contexts.get("v_neg_mask"),
+                                              contexts.get("v_pos_mask"), contexts.get("v_pos_mask")], v_ctx.shape[1]))
     audio = None
     if audio_state is not None:
         a_ctx = torch.cat([contexts["a_pos"], contexts["a_neg"], contexts["a_pos"], contexts["a_pos"]], dim=0)
         a_lat = audio_state.latent.repeat(n, 1, 1)
         audio = Modality(latent=a_lat, sigma=sigma_b,
                          timesteps=audio_state.denoise_mask.repeat(n, 1, 1) * sigma_b.view(n, 1, 1),
-                         positions=audio_state.positions.repeat(n, 1, 1, 1), context=a_ctx)
+                         positions=audio_state.positions.repeat(n, 1, 1, 1), context=a_ctx,
+                         context_mask=_cat_masks([contexts.get("a_pos_mask"), contexts.get("a_neg_mask"),
+                                                  contexts.get("a_pos_mask"), contexts.get("a_pos_mask")],
+                                                 a_ctx.shape[1]))
     a_blocks = list(a_params.stg_blocks) if a_params is not None else []
     keep = build_perturbation_config(cfg.num_layers, passes, list(v_params.stg_blocks), a_blocks, dev, dtype)
     vx, ax = model(video, audio, keep)

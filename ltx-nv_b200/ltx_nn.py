@@ -10,6 +10,8 @@ Layout choices that differ inside (not at the API):
   * RoPE tables are kept token-major, (T, H*d/2), shared by all samples whose positions
     agree; precompute_freqs_cis returns them as (B, H, T, d/2) views of that storage so
     callers see the reference's shapes.
+  * Attention and FeedForward modules may hold their weights in 8 bits as well
+    (quantize_fp8): their products then run on 8-bit rows (linear_fp8).
   * q, k, v and the gate logits of a self-attention are one packed (3D+H, D) weight:
     the module's own to_q / to_k / to_v / to_gate_logits parameters become views into
     it, so state_dict() is unchanged and nothing is stored twice.
@@ -252,6 +254,26 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
     return out
 
 
+def project(x, weight: torch.Tensor, weight8: Fp8Rows | None, out: torch.Tensor, epi: nat.Epilogue) -> None:
+    """out = epilogue(x W^T) of a module's projection: on 8-bit rows when the weight has an
+    8-bit form (x may then be 8-bit rows already), else in x's type."""
+    if weight8 is None:
+        nat.linear(x, weight, out, epi)
+    elif isinstance(x, Fp8Rows):
+        nat.linear_fp8(x, weight8, out, epi)
+    else:
+        nat.quantize_linear_fp8(x, weight8, out, epi)
+
+
+def norm_into(x: torch.Tensor, h: torch.Tensor, rows_per_batch: int, kind: int, eps: float,
+              mod: nat.Modulation | None, fp8: bool):
+    """norm_modulate of x (rows, D) as the operand of project: written to h, or as 8-bit rows."""
+    if fp8:
+        return nat.norm_modulate_fp8(x, rows_per_batch, kind, eps, mod)
+    nat.norm_modulate(x, h, rows_per_batch, kind, eps, mod)
+    return h
+
+
 # ---------------------------------------------------------------------------------------
 # RoPE (split type)
 # ---------------------------------------------------------------------------------------
@@ -480,6 +502,14 @@ class Attention(torch.nn.Module):
         self.to_v = torch.nn.Linear(context_dim, inner, bias=True)
         self.to_gate_logits = torch.nn.Linear(query_dim, heads, bias=True) if apply_gated_attention else None
         self.to_out = torch.nn.Linear(inner, query_dim, bias=True)
+        self.fp8: dict[str, Fp8Rows] = {}  # 8-bit weights by packing, after quantize_fp8
+
+    def quantize_fp8(self, packings: tuple[str, ...]) -> None:
+        """8-bit forms of the named packed weights ("self", or "q" and "kv") and of to_out,
+        used from now on; the parameters stay as they are."""
+        packed = {"self": self.packed_self, "q": self.packed_q, "kv": self.packed_kv}
+        self.fp8 = {name: quantize_fp8(packed[name]()[0]) for name in packings}
+        self.fp8["out"] = quantize_fp8(self.to_out.weight.detach())
 
     # packed weights -----------------------------------------------------------------
     def packed_self(self):
@@ -494,15 +524,15 @@ class Attention(torch.nn.Module):
         return _pack(self, ["to_k", "to_v"], "kv")
 
     # native core ----------------------------------------------------------------------
-    def project_qkv(self, x2: torch.Tensor, rows_per_batch: int, pe: RopeTables | None,
+    def project_qkv(self, x2, rows_per_batch: int, pe: RopeTables | None,
                     k_pe: RopeTables | None = None, normalize: bool = True) -> torch.Tensor:
-        """Self-attention projections of x2 (B*T, D) -> packed (B*T, 3I(+H)) buffer with
-        q and k normalised and rotated in place (normalize=False: left as projected, for a
-        caller that fuses the normalisation into its exchange)."""
+        """Self-attention projections of x2 (B*T, D), or its 8-bit rows, -> packed (B*T,
+        3I(+H)) buffer with q and k normalised and rotated in place (normalize=False: left as
+        projected, for a caller that fuses the normalisation into its exchange)."""
         inner = self.heads * self.dim_head
         w, b = self.packed_self()
-        qkv = torch.empty(x2.shape[0], w.shape[0], device=x2.device, dtype=x2.dtype)
-        nat.linear(x2, w, qkv, nat.epilogue(bias=b))
+        qkv = torch.empty(x2.shape[0], w.shape[0], device=w.device, dtype=w.dtype)
+        project(x2, w, self.fp8.get("self"), qkv, nat.epilogue(bias=b))
         if not normalize:
             return qkv
         if k_pe is None:
@@ -533,17 +563,28 @@ class Attention(torch.nn.Module):
                              else pe.sin, rope_ld_batch=pe.ld_batch)
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: torch.Tensor | None, batch: int,
-               tq: int, tk: int) -> torch.Tensor:
+               tq: int, tk: int, mask: torch.Tensor | None = None) -> torch.Tensor:
+        """mask: a key mask as nat.attention_masked takes it (key_mask)."""
         o = torch.empty(q.shape[0], self.heads * self.dim_head, device=q.device, dtype=q.dtype)
-        nat.attention(q, k, v, o, batch, tq, tk, self.heads, self.dim_head, self.dim_head ** -0.5, gate)
+        args = (q, k, v, o, batch, tq, tk, self.heads, self.dim_head, self.dim_head ** -0.5)
+        if mask is None:
+            nat.attention(*args, gate)
+        else:
+            nat.attention_masked(*args, mask, gate)
         return o
+
+    def project_out(self, o: torch.Tensor, out: torch.Tensor, epi: nat.Epilogue) -> None:
+        project(o, self.to_out.weight, self.fp8.get("out"), out, epi)
 
     def forward(self, x: torch.Tensor, context: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                 pe=None, k_pe=None, perturbation_mask: torch.Tensor | None = None,
                 all_perturbed: bool = False) -> torch.Tensor:
-        if mask is not None or perturbation_mask is not None or all_perturbed:
-            raise NotImplementedError("attention masks / STG perturbation are not supported yet")
+        """mask: over the keys (the context's tokens, or x's own), as sdpa takes it."""
+        if perturbation_mask is not None or all_perturbed:
+            raise NotImplementedError("STG perturbation is not supported yet")
         b, t, _ = x.shape
+        if mask is not None:
+            mask = key_mask(mask, b, t if context is None else context.shape[1])
         inner = self.heads * self.dim_head
         x2 = x.reshape(b * t, -1)
         pe_t = _tables_from_reference_layout(pe) if pe is not None else None
@@ -552,21 +593,21 @@ class Attention(torch.nn.Module):
         if context is None:
             qkv = self.project_qkv(x2, t, pe_t, kpe_t)
             o = self.attend(qkv[:, :inner], qkv[:, inner:2 * inner], qkv[:, 2 * inner:3 * inner],
-                            qkv[:, 3 * inner:] if gated else None, b, t, t)
+                            qkv[:, 3 * inner:] if gated else None, b, t, t, mask)
         else:
             s = context.shape[1]
             c2 = context.reshape(b * s, -1)
             wq, bq = self.packed_q()
             qg = torch.empty(b * t, wq.shape[0], device=x.device, dtype=x.dtype)
-            nat.linear(x2, wq, qg, nat.epilogue(bias=bq))
+            project(x2, wq, self.fp8.get("q"), qg, nat.epilogue(bias=bq))
             wkv, bkv = self.packed_kv()
             kv = torch.empty(b * s, 2 * inner, device=x.device, dtype=x.dtype)
-            nat.linear(c2, wkv, kv, nat.epilogue(bias=bkv))
+            project(c2, wkv, self.fp8.get("kv"), kv, nat.epilogue(bias=bkv))
             self._norm_rope(qg[:, :inner], t, self.q_norm.weight, pe_t)
             self._norm_rope(kv[:, :inner], s, self.k_norm.weight, kpe_t if kpe_t is not None else pe_t)
-            o = self.attend(qg[:, :inner], kv[:, :inner], kv[:, inner:], qg[:, inner:] if gated else None, b, t, s)
+            o = self.attend(qg[:, :inner], kv[:, :inner], kv[:, inner:], qg[:, inner:] if gated else None, b, t, s, mask)
         out = torch.empty(b * t, self.to_out.out_features, device=x.device, dtype=x.dtype)
-        nat.linear(o, self.to_out.weight, out, nat.epilogue(bias=self.to_out.bias))
+        self.project_out(o, out, nat.epilogue(bias=self.to_out.bias))
         return out.view(b, t, -1)
 
 
@@ -579,12 +620,20 @@ class FeedForward(torch.nn.Module):
         inner = int(dim * mult)
         self.proj_in = torch.nn.Linear(dim, inner, bias=bias)
         self.proj_out = torch.nn.Linear(inner, dim_out, bias=bias)
+        self.fp8: dict[str, Fp8Rows] = {}  # 8-bit weights, after quantize_fp8
+
+    def quantize_fp8(self) -> None:
+        """8-bit forms of both weights, used from now on; the parameters stay as they are."""
+        self.fp8 = {"in": quantize_fp8(self.proj_in.weight.detach()), "out": quantize_fp8(self.proj_out.weight.detach())}
+
+    def run(self, x2, out: torch.Tensor, epi: nat.Epilogue) -> None:
+        """out = epilogue(proj_out(gelu_tanh(proj_in(x2)))), x2 (rows, dim) or its 8-bit rows."""
+        h = torch.empty(out.shape[0], self.proj_in.out_features, device=out.device, dtype=out.dtype)
+        project(x2, self.proj_in.weight, self.fp8.get("in"), h, nat.epilogue(nat.EPI_GELU_TANH, bias=self.proj_in.bias))
+        project(h, self.proj_out.weight, self.fp8.get("out"), out, epi)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         b, t, d = x.shape
-        x2 = x.reshape(b * t, d)
-        h = torch.empty(b * t, self.proj_in.out_features, device=x.device, dtype=x.dtype)
-        nat.linear(x2, self.proj_in.weight, h, nat.epilogue(nat.EPI_GELU_TANH, bias=self.proj_in.bias))
         out = torch.empty(b * t, self.proj_out.out_features, device=x.device, dtype=x.dtype)
-        nat.linear(h, self.proj_out.weight, out, nat.epilogue(bias=self.proj_out.bias))
+        self.run(x.reshape(b * t, d), out, nat.epilogue(bias=self.proj_out.bias))
         return out.view(b, t, -1)

@@ -9,8 +9,9 @@ RMS norm. Same class names, constructor arguments and parameter names as the ref
 so its state dicts load unchanged.
 
 Every op is a libltxb200 kernel: ltx_register_fill, ltx_norm_modulate (RMS, no
-modulation), the packed QKV GEMM, q/k RMSNorm + RoPE, tcgen05 attention, out-projection
-and FFN GEMMs whose epilogues add the residual in place.
+modulation), the packed QKV GEMM, q/k RMSNorm + RoPE, tcgen05 attention (under the additive
+key mask where no registers replace the padding), out-projection and FFN GEMMs whose
+epilogues add the residual in place.
 """
 
 from __future__ import annotations
@@ -18,9 +19,16 @@ from __future__ import annotations
 import torch
 
 import _native as nat
-from ltx_nn import Attention, FeedForward, rope_tables
+from ltx_nn import Attention, FeedForward, key_mask, rope_tables
 
 NORM_EPS = 1e-6
+
+
+def _mask_of(additive_mask: torch.Tensor | None, batch: int, s: int) -> torch.Tensor | None:
+    """The key mask of an additive (B, 1, 1, S) mask; None where it adds nothing."""
+    if additive_mask is None or not bool((additive_mask != 0).any()):
+        return None
+    return key_mask(additive_mask, batch, s)
 
 
 class ConnectorBlock(torch.nn.Module):
@@ -31,15 +39,16 @@ class ConnectorBlock(torch.nn.Module):
         self.attn1 = Attention(dim, None, heads, dim_head, norm_eps, apply_gated_attention=gated)
         self.ff = FeedForward(dim, dim, bias=ff_bias)
 
-    def run(self, x: torch.Tensor, h: torch.Tensor, batch: int, s: int, pe) -> None:
-        """One block on the (B*S, D) residual stream x, updated in place; h is scratch."""
+    def run(self, x: torch.Tensor, h: torch.Tensor, batch: int, s: int, pe, mask: torch.Tensor | None = None) -> None:
+        """One block on the (B*S, D) residual stream x, updated in place; h is scratch; mask:
+        a key mask (ltx_nn.key_mask) of the tokens, or None."""
         attn, ff = self.attn1, self.ff
         inner = attn.heads * attn.dim_head
         nat.norm_modulate(x, h, s, nat.LTX_NORM_RMS, NORM_EPS, None)
         qkv = attn.project_qkv(h, s, pe)
         gated = attn.to_gate_logits is not None
         o = attn.attend(qkv[:, :inner], qkv[:, inner:2 * inner], qkv[:, 2 * inner:3 * inner],
-                        qkv[:, 3 * inner:3 * inner + attn.heads] if gated else None, batch, s, s)
+                        qkv[:, 3 * inner:3 * inner + attn.heads] if gated else None, batch, s, s, mask)
         nat.linear(o, attn.to_out.weight, x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn.to_out.bias, residual=x,
                                                           rows_per_batch=s))
         nat.norm_modulate(x, h, s, nat.LTX_NORM_RMS, NORM_EPS, None)
@@ -49,12 +58,10 @@ class ConnectorBlock(torch.nn.Module):
                                                           rows_per_batch=s))
 
     def forward(self, x: torch.Tensor, additive_mask=None, pe=None) -> torch.Tensor:
-        if additive_mask is not None and bool((additive_mask != 0).any()):
-            raise NotImplementedError("additive attention masks (connectors without registers)")
         b, s, d = x.shape
         xs = x.reshape(b * s, d).contiguous().clone()
         h = torch.empty_like(xs)
-        self.run(xs, h, b, s, pe)
+        self.run(xs, h, b, s, pe, _mask_of(additive_mask, b, s))
         return xs.view(b, s, d)
 
 
@@ -97,14 +104,14 @@ class Embeddings1DConnector(torch.nn.Module):
                               additive_mask.to(hidden_states.dtype).reshape(b * s).contiguous(),
                               self.learnable_registers.to(hidden_states.dtype), s, x)
             additive_mask = torch.zeros_like(additive_mask)
+            mask = None
         else:
-            if bool((additive_mask != 0).any()):
-                raise NotImplementedError("additive attention masks (connectors without registers)")
+            mask = _mask_of(additive_mask, b, s)
             x.copy_(hidden_states.reshape(b * s, d))
         pe = self._pe(s, hidden_states.device, hidden_states.dtype)
         h = torch.empty_like(x)
         for blk in self.blocks:
-            blk.run(x, h, b, s, pe)
+            blk.run(x, h, b, s, pe, mask)
         out = torch.empty_like(x)
         nat.norm_modulate(x, out, s, nat.LTX_NORM_RMS, NORM_EPS, None)
         return out.view(b, s, d), additive_mask
