@@ -571,8 +571,8 @@ def attention_merge(o_parts: torch.Tensor, lse_parts: torch.Tensor, gate_logits:
 def _on(t: torch.Tensor, name: str, *args, label: str | None = None) -> None:
     """_call with the stream of t's device appended, made on that device (which need not be
     the current one)."""
-    dev = t.device.index
-    if dev == torch.cuda.current_device():
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
         _call(name, *args, torch._C._cuda_getCurrentRawStream(dev), label=label)
         return
     with torch.cuda.device(dev):
@@ -580,10 +580,11 @@ def _on(t: torch.Tensor, name: str, *args, label: str | None = None) -> None:
 
 
 def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
-    if not first.is_cuda:
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("libltxb200 kernels take CUDA tensors only")
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
 
 
@@ -668,10 +669,10 @@ def norm_modulate_fp8(x: torch.Tensor, rows_per_batch: int, kind: int, eps: floa
 
 def linear_fp8(a: Fp8Rows, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = None) -> None:
     """c = epilogue(a @ w.T (+ bias)); a (M, K) and w (N, K) 8-bit rows, c (M, N) a row-major
-    view in the epilogue's type."""
-    if a.cols != w.cols or tuple(c.shape) != (a.rows, w.rows):
+    view in the epilogue's type, or any contiguous (..., N) tensor of M rows."""
+    if a.cols != w.cols or c.shape[-1] != w.rows or c.numel() != a.rows * w.rows:
         raise ValueError(f"shape mismatch a{a.shape} w{w.shape} c{tuple(c.shape)}")
-    dt, ld = _dt(c), _ld(c)
+    dt, ld = _dt(c), (w.rows if c.is_contiguous() else _ld(c))
     _same_device(c, a.data, w.data)
     if c.numel():
         _on(c, "ltx_linear_fp8", a.data.data_ptr(), a.data.stride(0), a.scales.data_ptr(), w.data.data_ptr(),
@@ -687,11 +688,12 @@ def fp8_force_pair(pair: int) -> None:
 
 def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = None) -> None:
     """c = epilogue(quantize_fp8(x) @ w.T (+ bias)); x (M, K) float32 or bfloat16 with unit
-    column stride, c (M, N) a row-major view in the epilogue's type."""
+    column stride, c (M, N) a row-major view in the epilogue's type, or any contiguous (..., N)
+    tensor of M rows."""
     m, k = x.shape
-    if k != w.cols or tuple(c.shape) != (m, w.rows):
+    if k != w.cols or c.shape[-1] != w.rows or c.numel() != m * w.rows:
         raise ValueError(f"shape mismatch x{tuple(x.shape)} w{w.shape} c{tuple(c.shape)}")
-    xdt, ldx, dt, ld = _dt(x), _ld(x), _dt(c), _ld(c)
+    xdt, ldx, dt, ld = _dt(x), _ld(x), _dt(c), (w.rows if c.is_contiguous() else _ld(c))
     _same_device(x, c, w.data)
     if not c.numel():
         return
@@ -711,23 +713,33 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch
                      gate_logits: torch.Tensor | None = None) -> None:
     """attention with a key mask (batch, tk), or (1, tk) for all samples: bool (True: the key
     takes part) or an additive float32 / bfloat16 one."""
-    if mask.dtype not in MASK_KINDS:
-        raise TypeError(f"unsupported mask dtype {mask.dtype}; bool, float32 or bfloat16")
     if mask.dim() != 2 or mask.shape[1] != tk or mask.shape[0] not in (1, batch) or (tk > 1 and mask.stride(1) != 1):
         raise ValueError(f"mask must be a row-major ({batch} or 1, {tk}) view, got {tuple(mask.shape)}")
-    dt = _dt(q)
     for name, t, rows in (("k", k, batch * tk), ("v", v, batch * tk), ("o", o, batch * tq), ("q", q, batch * tq)):
-        if t.dtype != q.dtype:
-            raise TypeError(f"{name} is {t.dtype}, q is {q.dtype}")
         if t.shape[0] != rows or t.shape[1] < heads * head_dim:
             raise ValueError(f"{name} must have {rows} rows of at least {heads * head_dim} columns")
-    if gate_logits is not None and (gate_logits.dtype != q.dtype or gate_logits.shape[0] != batch * tq
-                                    or gate_logits.shape[1] < heads):
-        raise ValueError(f"gate_logits must be {q.dtype} ({batch * tq}, >= {heads})")
+    if gate_logits is not None and (gate_logits.shape[0] != batch * tq or gate_logits.shape[1] < heads):
+        raise ValueError(f"gate_logits must be ({batch * tq}, >= {heads})")
+    attention_masked_rows(q, _ld(q), k, _ld(k), v, _ld(v), o, _ld(o), batch, tq, tk, heads, head_dim, scale, mask,
+                          gate_logits, _ld(gate_logits) if gate_logits is not None else 0)
+
+
+def attention_masked_rows(q: torch.Tensor, ldq: int, k: torch.Tensor, ldk: int, v: torch.Tensor, ldv: int,
+                          o: torch.Tensor, ldo: int, batch: int, tq: int, tk: int, heads: int, head_dim: int,
+                          scale: float, mask: torch.Tensor, gate_logits: torch.Tensor | None, ld_gate: int) -> None:
+    """attention_masked of tensors whose shapes the caller has checked, as row strides of
+    their token-major rows, without the 2-D views."""
+    dt = _dt(q)
+    if mask.dtype not in MASK_KINDS:
+        raise TypeError(f"unsupported mask dtype {mask.dtype}; bool, float32 or bfloat16")
+    if k.dtype != q.dtype or v.dtype != q.dtype or o.dtype != q.dtype:
+        raise TypeError(f"q is {q.dtype}, k {k.dtype}, v {v.dtype}, o {o.dtype}")
+    if gate_logits is not None and gate_logits.dtype != q.dtype:
+        raise TypeError(f"gate_logits is {gate_logits.dtype}, q is {q.dtype}")
     _same_device(q, k, v, o, mask, gate_logits)
-    _on(q, "ltx_attention_masked", q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), o.data_ptr(), _ld(o),
-        batch, tq, tk, heads, head_dim, scale, mask.data_ptr(), 0 if mask.shape[0] == 1 else mask.stride(0),
-        MASK_KINDS[mask.dtype], _ptr(gate_logits), _ld(gate_logits) if gate_logits is not None else 0, dt,
+    _on(q, "ltx_attention_masked", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), ldo, batch, tq,
+        tk, heads, head_dim, scale, mask.data_ptr(), 0 if mask.shape[0] == 1 else mask.stride(0),
+        MASK_KINDS[mask.dtype], gate_logits.data_ptr() if gate_logits is not None else None, ld_gate, dt,
         label=f"attention_masked B={batch} H={heads} Tq={tq} Tk={tk} d={head_dim}" if _profile is not None else None)
 
 

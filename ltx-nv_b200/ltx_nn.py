@@ -83,11 +83,23 @@ def key_mask(mask: torch.Tensor, batch: int, tk: int) -> torch.Tensor:
 
 
 def _row_major(x: torch.Tensor) -> torch.Tensor:
-    """x (B, T, W) as a (B * T, W) row-major view; a copy only where there is no such view."""
-    if x.dim() != 3:
-        raise ValueError(f"expected (batch, tokens, width), got {tuple(x.shape)}")
+    """x (..., W) as a (rows, W) row-major view; a copy only where there is no such view, or
+    where its rows overlap (expanded tensors)."""
     x2 = x.reshape(-1, x.shape[-1])
-    return x2 if x2.stride(1) == 1 else x2.contiguous()
+    if x2.stride(1) == 1 and x2.stride(0) >= x2.shape[1]:
+        return x2
+    return x2.clone(memory_format=torch.contiguous_format)  # contiguous() keeps a single row's odd strides
+
+
+def _token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x (B, T, W) as a tensor and its row stride: x itself where its B * T rows are evenly
+    spaced, without the cost of a view; else _row_major's."""
+    b, t, w = x.shape
+    sb, st, sw = x.stride()
+    if sw == 1 and t > 1 and st >= w and (b == 1 or sb == t * st):
+        return x, st
+    x2 = _row_major(x)
+    return x2, x2.stride(0)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int,
@@ -107,9 +119,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     tk = k.shape[1]
     if heads <= 0 or width % heads:
         raise ValueError(f"the width {width} is not a multiple of {heads} heads")
-    if tuple(k.shape) != (b, tk, width) or tuple(v.shape) != (b, tk, width):
+    if k.shape != (b, tk, width) or v.shape != (b, tk, width):
         raise ValueError(f"k and v must be ({b}, Tk, {width}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    if gate_logits is not None and tuple(gate_logits.shape) != (b, tq, heads):
+    if gate_logits is not None and gate_logits.shape != (b, tq, heads):
         raise ValueError(f"gate_logits must be ({b}, {tq}, {heads}), got {tuple(gate_logits.shape)}")
     if out is None:
         out = torch.empty(b, tq, width, device=q.device, dtype=q.dtype)
@@ -122,13 +134,13 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     if tk == 0:
         return out.zero_()
     d = width // heads
-    g = _row_major(gate_logits) if gate_logits is not None else None
-    args = (_row_major(q), _row_major(k), _row_major(v), out.view(b * tq, width), b, tq, tk, heads, d,
-            d ** -0.5 if scale is None else float(scale))
+    scale = d ** -0.5 if scale is None else float(scale)
     if mask is None:
-        nat.attention(*args, g)
+        nat.attention(_row_major(q), _row_major(k), _row_major(v), out.view(b * tq, width), b, tq, tk, heads, d, scale,
+                      _row_major(gate_logits) if gate_logits is not None else None)
     else:
-        nat.attention_masked(*args, mask, g)
+        nat.attention_masked_rows(*_token_rows(q), *_token_rows(k), *_token_rows(v), out, width, b, tq, tk, heads, d,
+                                  scale, mask, *(_token_rows(gate_logits) if gate_logits is not None else (None, 0)))
     return out
 
 
@@ -140,8 +152,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     """x (..., K) float32 or bfloat16 -> its 8-bit rows: e4m3 values with a power-of-two scale
     per 128 columns. Weights (N, K) are quantised with it once."""
-    x2 = x.reshape(-1, x.shape[-1])
-    return nat.quantize_fp8(x2 if x2.stride(1) == 1 else x2.contiguous(), x.shape)
+    return nat.quantize_fp8(_row_major(x), x.shape)
 
 
 def _modulation(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None):
@@ -149,32 +160,30 @@ def _modulation(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor
     and the tensors that it points to. One descriptor addresses both vectors from the lower
     of their addresses, with one stride; vectors that do not share it are copied."""
     b, t, d = x.shape
-    held = {}
-    for name, vec in (("shift", shift), ("scale", scale)):
-        if vec is None:
-            continue
-        if tuple(vec.shape) not in ((b, d), (b, t, d)) or any(v.dim() != vec.dim() for v in held.values()):
-            raise ValueError(f"{name} must be ({b}, {d}) or ({b}, {t}, {d}), like the other vector, got "
+    vecs = [v for v in (shift, scale) if v is not None]
+    if not vecs:
+        return None, vecs
+    first = vecs[0]
+    for vec in vecs:
+        if vec.shape != first.shape or vec.shape not in ((b, d), (b, t, d)):
+            raise ValueError(f"shift and scale must be ({b}, {d}) or ({b}, {t}, {d}), one like the other, got "
                              f"{tuple(vec.shape)}")
-        if vec.dtype != x.dtype or vec.device != x.device:
-            raise ValueError(f"{name} must be {x.dtype} on {x.device}")
-        held[name] = vec
-    if not held:
-        return None, held
-    vecs = list(held.values())
-    st = vecs[0].stride()
-    if any(v.stride() != st or v.stride(-1) != 1 or v.data_ptr() % 32 for v in vecs) or any(i % 8 for i in st[:-1]):
-        held = {name: torch.empty(vec.shape, dtype=vec.dtype, device=vec.device).copy_(vec)
-                for name, vec in held.items()}
-        st = next(iter(held.values())).stride()
-    base = min(v.data_ptr() for v in held.values())
+        if vec.dtype != x.dtype or vec.get_device() != x.get_device():
+            raise ValueError(f"shift and scale must be {x.dtype} on {x.device}")
+    st = first.stride()
+    if any([v.stride() != st or v.data_ptr() % 32 for v in vecs]) or st[-1] != 1 or any([i % 8 for i in st[:-1]]):
+        vecs = [torch.empty(v.shape, dtype=v.dtype, device=v.device).copy_(v) for v in vecs]
+        st = vecs[0].stride()
+    ptrs = [v.data_ptr() for v in vecs]
     m = nat.Modulation()
-    m.mod = base
+    m.mod = base = min(ptrs)
     m.mod_ld_batch, m.mod_ld_tok = st[0], (st[1] if len(st) == 3 else 0)
-    for name, vec in held.items():
-        setattr(m, "has_" + name, 1)
-        setattr(m, name + "_mod_off", (vec.data_ptr() - base) // vec.element_size())
-    return m, held
+    size = x.element_size()
+    if shift is not None:
+        m.has_shift, m.shift_mod_off = 1, (ptrs[0] - base) // size
+    if scale is not None:
+        m.has_scale, m.scale_mod_off = 1, (ptrs[-1] - base) // size
+    return m, vecs
 
 
 _NORM_KINDS = {"rms": nat.LTX_NORM_RMS, "layer": nat.LTX_NORM_LAYER, "none": nat.LTX_NORM_NONE}
@@ -186,6 +195,8 @@ def norm_modulate_fp8(x: torch.Tensor, scale: torch.Tensor | None = None, shift:
     type; kind "rms", "layer" or "none"; D a multiple of 8."""
     if kind not in _NORM_KINDS:
         raise ValueError(f"kind must be one of {sorted(_NORM_KINDS)}, got {kind!r}")
+    if x.dim() != 3:
+        raise ValueError(f"expected (batch, tokens, width), got {tuple(x.shape)}")
     x2 = _row_major(x)
     mod, held = _modulation(x, shift, scale)
     out = nat.norm_modulate_fp8(x2, max(x.shape[1], 1), _NORM_KINDS[kind], eps, mod, x.shape)
@@ -220,37 +231,36 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
         dtype = x.dtype if isinstance(x, torch.Tensor) else residual.dtype if residual is not None else torch.bfloat16
     if x.shape[-1] != weight.cols or len(weight.shape) != 2:
         raise ValueError(f"x has {x.shape[-1]} columns, the weight is {weight.shape}")
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     shape = (*lead, n)
+    dev = x.device
     for name, t, want in (("bias", bias, (n,)), ("residual", residual, shape), ("out", out, shape)):
-        if t is not None and (tuple(t.shape) != want or t.dtype != dtype or t.device != x.device):
-            raise ValueError(f"{name} must be {dtype} {want} on {x.device}, got {t.dtype} {tuple(t.shape)}")
+        if t is not None and (t.shape != want or t.dtype != dtype or t.device != dev):
+            raise ValueError(f"{name} must be {dtype} {want} on {dev}, got {t.dtype} {tuple(t.shape)}")
     kind, rpb, mod = _ACTIVATIONS[activation], 1, None
     if residual is not None:
         kind = nat.EPI_GATE_RESIDUAL
-        residual2 = residual.reshape(-1, n)
-        residual2 = residual2 if residual2.stride(1) == 1 else residual2.contiguous()
+        residual2 = _row_major(residual)
         if gate is not None:
             if residual.dim() != 3 or tuple(gate.shape) not in ((lead[0], n), shape):
                 raise ValueError(f"gate must be (B, N) or (B, T, N) of a (B, T, N) residual, got {tuple(gate.shape)}")
-            if gate.dtype != dtype or gate.device != x.device:
-                raise ValueError(f"gate must be {dtype} on {x.device}")
+            if gate.dtype != dtype or gate.device != dev:
+                raise ValueError(f"gate must be {dtype} on {dev}")
             gate = gate.contiguous()
             rpb = max(lead[1], 1)
             per_tok = gate.dim() == 3
             mod = nat.modulation(None, gate, shift=None, scale=(0, 0), mod_ld_batch=rpb * n if per_tok else n,
                                  mod_ld_tok=n if per_tok else 0)
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=dtype)
+        out = torch.empty(shape, device=dev, dtype=dtype)
     elif not out.is_contiguous():
         raise ValueError("out must be contiguous")
     epi = nat.epilogue(kind, bias=bias.contiguous() if bias is not None else None,
                        residual=residual2 if residual is not None else None, gate=mod, rows_per_batch=rpb)
     if isinstance(x, Fp8Rows):
-        nat.linear_fp8(x, weight, out.view(-1, n), epi)
+        nat.linear_fp8(x, weight, out, epi)
     elif weight.cols:
-        x2 = x.reshape(-1, weight.cols)
-        nat.quantize_linear_fp8(x2 if x2.stride(1) == 1 else x2.contiguous(), weight, out.view(-1, n), epi)
+        nat.quantize_linear_fp8(_row_major(x), weight, out, epi)
     return out
 
 
