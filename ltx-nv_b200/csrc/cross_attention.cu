@@ -97,6 +97,268 @@ __global__ void __launch_bounds__(128) masked_attn_simt_kernel(const T* __restri
 }
 
 // ---------------------------------------------------------------------------------
+// Few queries (serving's single tokens), bound by the bytes of K and V: a unit is (sample,
+// head, one query or four), and its kept keys are streamed once, straight from memory to
+// registers. A warp takes 32 keys at a time: their masks in one load (the next ones' ahead
+// of the arithmetic), then K and V in pieces of 8 columns a lane, D / 8 lanes to a key, BATCH
+// keys a lane in flight; a left-out key is not read at all. Scores, statistics and sums are
+// fp32; every group of D / 8 lanes keeps its own running maximum, and groups, warps and the
+// CTAs of a cluster that share a unit's keys are joined at the end in a fixed order. 2 x 32
+// heads of 128, 4096 keys, one query: 134 MB in 27.9 us, 4.8 TB/s.
+// ---------------------------------------------------------------------------------
+// Queries of a unit: 1, or up to 4 that share the loads and the conversions of a key.
+// (2 samples, 32 heads of 128, 4096 keys, one query: 4 warps with 8 keys a lane 28.4 us, 4
+// keys 34.9, 8 warps with 4 keys 35.6; four queries: 8 warps with 4 keys 54.5, 4 warps 61.1.)
+constexpr int few_warps(int queries) { return queries == 1 ? 4 : 8; }
+
+template <typename T>
+LTX_DEVICE float few_exp2(float x) {
+  return std::is_same<T, float>::value ? exp2f(x) : ex2_approx(x);
+}
+
+LTX_DEVICE uint4 few_load(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+LTX_DEVICE void few_load8(const __nv_bfloat16* p, uint4 (&r)[1]) { r[0] = few_load(p); }
+LTX_DEVICE void few_load8(const float* p, uint4 (&r)[2]) {
+  r[0] = few_load(p);
+  r[1] = few_load(p + 4);
+}
+LTX_DEVICE void few_values(const uint4 (&r)[1], float (&v)[8]) {
+  const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+LTX_DEVICE void few_values(const uint4 (&r)[2], float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[4 * i] = __uint_as_float(r[i].x);
+    v[4 * i + 1] = __uint_as_float(r[i].y);
+    v[4 * i + 2] = __uint_as_float(r[i].z);
+    v[4 * i + 3] = __uint_as_float(r[i].w);
+  }
+}
+
+template <typename T, int D, int QN>
+__global__ void __launch_bounds__(few_warps(QN) * 32, QN == 1 ? 4 : 2)
+    masked_attn_few_kernel(const T* Q, int64_t ldq, const T* K, int64_t ldk, const T* V, int64_t ldv, T* O,
+                           int64_t ldo, int Tq, int Tk, int H, int split, float scale_log2, KeyMask mask,
+                           const T* gate, int64_t ld_gate) {
+  constexpr int LG = D / 8, G = 32 / LG;  // lanes of a key, keys of a warp at a time
+  constexpr int REGS = sizeof(T) / 2;     // 16-byte registers of 8 columns
+  constexpr int BATCH = (QN == 1 ? 8 : 4) / REGS;
+  constexpr int PARTS = QN * D, WARPS = few_warps(QN);
+  __shared__ float part_o[WARPS][PARTS], part_ml[WARPS][QN][2];
+  __shared__ float cta_o[PARTS], cta_ml[QN][2];
+  const int lane = lane_id(), warp = warp_id(), group = lane / LG, col = lane % LG * 8;
+  const int unit = int(blockIdx.x) / split, rank = int(blockIdx.x) % split;
+  const int h = unit % H, nq = (Tq + QN - 1) / QN, q0 = unit / H % nq * QN;
+  const int64_t b = unit / H / nq, qrow = b * Tq + q0;
+  const int queries = min(QN, Tq - q0);
+  pdl_wait();
+  pdl_trigger();
+
+  const T* kp = K + b * Tk * ldk + int64_t(h) * D + col;
+  const T* vp = V + b * Tk * ldv + int64_t(h) * D + col;
+  const int64_t step = int64_t(split) * WARPS * 32;
+  auto bias_at = [&](int64_t t) { return t < Tk ? mask.at(b, t) * 1.4426950408889634f : -INFINITY; };
+  int64_t t0 = (int64_t(rank) * WARPS + warp) * 32;
+  float next = bias_at(t0 + lane);
+  float q[QN][8], acc[QN][8], m[QN], l[QN];
+#pragma unroll
+  for (int n = 0; n < QN; ++n) {  // queries past the last repeat it, and are not stored
+    uint4 r[REGS];
+    few_load8(Q + (qrow + min(n, queries - 1)) * ldq + int64_t(h) * D + col, r);
+    few_values(r, q[n]);
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[n][e] *= scale_log2;
+      acc[n][e] = 0.f;
+    }
+  }
+  for (; t0 < Tk; t0 += step) {
+    const float bias = next;
+    next = bias_at(t0 + step + lane);
+    const uint32_t kept = __ballot_sync(0xffffffffu, bias != -INFINITY);
+#pragma unroll
+    for (int j = 0; j < 32 / G; j += BATCH) {
+      if ((kept >> (j * G) & (BATCH * G == 32 ? 0xffffffffu : (1u << (BATCH * G % 32)) - 1u)) == 0) continue;
+      uint4 kr[BATCH][REGS], vr[BATCH][REGS];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = (j + i) * G + group;
+#pragma unroll
+        for (int w = 0; w < REGS; ++w) kr[i][w] = vr[i][w] = make_uint4(0, 0, 0, 0);
+        if (kept >> r & 1u) {
+          few_load8(kp + (t0 + r) * ldk, kr[i]);
+          few_load8(vp + (t0 + r) * ldv, vr[i]);
+        }
+      }
+      float sc[QN][BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        float kv[8];
+        few_values(kr[i], kv);
+#pragma unroll
+        for (int n = 0; n < QN; ++n) {
+          sc[n][i] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sc[n][i] = fmaf(q[n][e], kv[e], sc[n][i]);
+        }
+      }
+#pragma unroll
+      for (int off = LG / 2; off > 0; off /= 2)
+#pragma unroll
+        for (int n = 0; n < QN; ++n)
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) sc[n][i] += __shfl_xor_sync(0xffffffffu, sc[n][i], off);
+      float add[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) add[i] = __shfl_sync(0xffffffffu, bias, (j + i) * G + group);
+#pragma unroll
+      for (int n = 0; n < QN; ++n) {
+        float mx = m[n];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          sc[n][i] = add[i] == -INFINITY ? -INFINITY : sc[n][i] + add[i];
+          mx = fmaxf(mx, sc[n][i]);
+        }
+        const float ref = mx == -INFINITY ? 0.f : mx, alpha = few_exp2<T>(m[n] - ref);
+        m[n] = mx;
+        l[n] *= alpha;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[n][e] *= alpha;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          sc[n][i] = few_exp2<T>(sc[n][i] - ref);
+          l[n] += sc[n][i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        float vv[8];
+        few_values(vr[i], vv);
+#pragma unroll
+        for (int n = 0; n < QN; ++n)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[n][e] = fmaf(sc[n][i], vv[e], acc[n][e]);
+      }
+    }
+  }
+
+  // join the groups of a warp, ...
+#pragma unroll
+  for (int n = 0; n < QN; ++n) {
+#pragma unroll
+    for (int off = LG; off < 32; off *= 2) {
+      const float mo = __shfl_xor_sync(0xffffffffu, m[n], off), lo = __shfl_xor_sync(0xffffffffu, l[n], off);
+      const float mx = fmaxf(m[n], mo), ref = mx == -INFINITY ? 0.f : mx;
+      const float f = few_exp2<T>(m[n] - ref), fo = few_exp2<T>(mo - ref);
+      l[n] = l[n] * f + lo * fo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[n][e] = acc[n][e] * f + __shfl_xor_sync(0xffffffffu, acc[n][e], off) * fo;
+      m[n] = mx;
+    }
+    if (lane < LG) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part_o[warp][n * D + col + e] = acc[n][e];
+      if (lane == 0) part_ml[warp][n][0] = m[n], part_ml[warp][n][1] = l[n];
+    }
+  }
+  __syncthreads();
+  // ... the warps, ...
+  for (int i = threadIdx.x; i < queries * D; i += WARPS * 32) {
+    const int n = i / D;
+    float o = 0.f, L = 0.f, M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, part_ml[w][n][0]);
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = few_exp2<T>(part_ml[w][n][0] - ref);
+      L += part_ml[w][n][1] * f;
+      o += part_o[w][i] * f;
+    }
+    if (split == 1) {
+      float g = 1.f;
+      if (gate != nullptr) g = 2.f / (1.f + expf(-ld_elem<T>(gate + (qrow + n) * ld_gate + h)));
+      st_elem<T>(O + (qrow + n) * ldo + int64_t(h) * D + i % D, L == 0.f ? 0.f : o * (g / L));
+    } else {
+      cta_o[i] = o;
+      if (i % D == 0) cta_ml[n][0] = M, cta_ml[n][1] = L;
+    }
+  }
+  if (split == 1) return;
+  // ... and the CTAs of a cluster (each takes its share of the columns).
+  cluster_sync_all();
+  for (int i = rank * WARPS * 32 + threadIdx.x; i < queries * D; i += split * WARPS * 32) {
+    const int n = i / D;
+    float po[8], pm[8], pl[8], M = -INFINITY, o = 0.f, L = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      pm[r] = -INFINITY, pl[r] = po[r] = 0.f;
+      if (r < split) {
+        pm[r] = ld_cluster_f1(mapa_shared(smem_u32(&cta_ml[n][0]), r));
+        pl[r] = ld_cluster_f1(mapa_shared(smem_u32(&cta_ml[n][1]), r));
+        po[r] = ld_cluster_f1(mapa_shared(smem_u32(&cta_o[i]), r));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) M = fmaxf(M, pm[r]);
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float f = few_exp2<T>(pm[r] - ref);
+      o += po[r] * f;
+      L += pl[r] * f;
+    }
+    float g = 1.f;
+    if (gate != nullptr) g = 2.f / (1.f + expf(-ld_elem<T>(gate + (qrow + n) * ld_gate + h)));
+    st_elem<T>(O + (qrow + n) * ldo + int64_t(h) * D + i % D, L == 0.f ? 0.f : o * (g / L));
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its sums
+}
+
+// bf16: for up to 4 queries a sample, where a unit of the tensor-core kernel would be one row
+// of 256 (2 samples, 32 heads of 128, 64 / 1024 / 4096 keys: one query 4.0 / 10.3 / 27.9 us
+// against 8.5 / 21.8 / 57.2, four 7.5 / 16.2 / 54.3 against 8.4 / 22.1 / 57.2, eight 7.8 / 28.7
+// / 99.2 against 8.5 / 22.1 / 57.5).
+// fp32: while the kernel of one query per thread would leave SMs without a block, or at 128
+// columns a head, where its accumulators do not stay in registers, with four of them (heads
+// of 64: 1 x 8 heads, 200 keys, 480 queries 29 us against 96; 2 x 8, 256, 1024 112 / 118; 2 x
+// 16, 256, 1024 218 / 150. Heads of 128: 46 / 333, 181 / 418, 357 / 465; 2 x 32, 128, 6144
+// 3238 / 2780).
+inline bool use_few(int64_t B, int64_t Tq, int H, int D, bool bf16) {
+  if (B * Tq * H >= int64_t(1) << 27) return false;
+  return bf16 ? Tq <= 4 : Tq <= 4 || B * H * ((Tq + 127) / 128) < num_sms() * (D == 128 ? 4 : 1);
+}
+
+template <typename T, int D>
+void launch_masked_few(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
+                       int64_t ldo, int B, int64_t Tq, int64_t Tk, int H, float scale, const KeyMask& mask,
+                       const void* gate, int64_t ld_gate, cudaStream_t s) {
+  const bool one = Tq == 1;
+  const int64_t units = int64_t(B) * (one ? 1 : (Tq + 3) / 4) * H;
+  const int warps = one ? few_warps(1) : few_warps(4);
+  // Up to 32 warps for every SM, while every warp still has a chunk of 32 keys.
+  int split = 1;
+  while (split < 8 && units * split * warps < 32 * num_sms() && Tk > int64_t(split) * warps * 32) split *= 2;
+  launch_pdl(one ? masked_attn_few_kernel<T, D, 1> : masked_attn_few_kernel<T, D, 4>, dim3(unsigned(units * split)),
+             dim3(warps * 32), 0, s, unsigned(split), static_cast<const T*>(q), ldq, static_cast<const T*>(k), ldk,
+             static_cast<const T*>(v), ldv, static_cast<T*>(o), ldo, int(Tq), int(Tk), H, split,
+             scale * 1.4426950408889634f, mask, static_cast<const T*>(gate), ld_gate);
+}
+
+// ---------------------------------------------------------------------------------
 // bf16: persistent tcgen05 kernel. A unit is (sample, head, 256 queries) = two 128-row Q
 // tiles; CTAs walk the units in steps of the grid, and every role runs straight on from
 // one unit to the next, so a unit's Q load, first Q K^T and output store overlap its
@@ -819,7 +1081,19 @@ extern "C" int ltx_attention_masked(const void* q, int64_t ldq, const void* k, i
         qp, ldq, static_cast<const T*>(k), ldk, static_cast<const T*>(v), ldv, static_cast<T*>(o), ldo, int(Tq),
         int(Tk), scale, km, static_cast<const T*>(gate_logits), ld_gate), note_launch();
   };
-  if (dtype == LTX_F32) {
+  if (use_few(B, Tq, heads, head_dim, dtype == LTX_BF16)) {
+    const auto few = [&](auto elem, auto dim) {
+      launch_masked_few<decltype(elem), decltype(dim)::value>(q, ldq, k, ldk, v, ldv, o, ldo, B, Tq, Tk, heads, scale,
+                                                              km, gate_logits, ld_gate, s);
+    };
+    if (dtype == LTX_BF16)
+      head_dim == 64 ? few(__nv_bfloat16{}, std::integral_constant<int, 64>{})
+                     : few(__nv_bfloat16{}, std::integral_constant<int, 128>{});
+    else if (head_dim == 32)
+      few(0.f, std::integral_constant<int, 32>{});
+    else
+      head_dim == 64 ? few(0.f, std::integral_constant<int, 64>{}) : few(0.f, std::integral_constant<int, 128>{});
+  } else if (dtype == LTX_F32) {
     auto qp = static_cast<const float*>(q);
     if (head_dim == 32)
       run(qp, std::integral_constant<int, 32>{});

@@ -218,3 +218,59 @@ def test_a_sample_does_not_depend_on_its_batch():
         one = ltx_nn.cross_attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], h, mask=m[i:i + 1])
         err = (one.double() - whole[i:i + 1].double()).abs()
         assert (err <= whole[i:i + 1].double().abs() * 2.0 ** -7 + 2.0 ** -9).all()
+
+
+# Few queries: one, or groups of four with a last one that is not full; keys that end inside
+# a chunk of 32, contexts of one chunk up to many for every warp of a cluster's eight CTAs,
+# and more units than a wave of CTAs.
+FEW = [(1, 1, 1, 1), (2, 1, 31, 3), (1, 4, 33, 2), (3, 3, 129, 4), (2, 2, 255, 5), (1, 1, 1030, 2), (2, 4, 2049, 1),
+       (1, 1, 9001, 1), (70, 1, 70, 9), (40, 3, 260, 16)]
+
+
+@pytest.mark.parametrize("kind", ["right", "holes", "all", "one"])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 32),
+                                     (torch.float32, 64), (torch.float32, 128)])
+@pytest.mark.parametrize("b,tq,tk,h", FEW)
+def test_few_queries(b, tq, tk, h, dtype, d, kind):
+    g, q, k, v, gate = inputs(b + 3 * tq + tk + h, b, tq, tk, h, d, dtype)
+    m = mask_of(kind, g, b, tk)
+    out = torch.full((b, tq, h * d), 5.0, device=DEV, dtype=dtype)
+    got = ltx_nn.cross_attention(q, k, v, h, mask=m, gate_logits=gate, out=out)
+    assert got is out
+    check(got, q, k, v, h, ~m, None, gate, d ** -0.5)
+
+
+@pytest.mark.parametrize("b,tq,tk,h,d", [(10, 129, 70, 8, 64), (19, 5, 33, 8, 32), (20, 129, 40, 15, 128), (2, 600, 129, 2, 64),
+                                         (1, 300, 70, 3, 32)])
+def test_fp32_with_many_and_few_blocks(b, tq, tk, h, d):
+    g, q, k, v, gate = inputs(17, b, tq, tk, h, d, torch.float32)
+    m = mask_of("holes", g, b, tk)
+    check(ltx_nn.cross_attention(q, k, v, h, mask=m, gate_logits=gate), q, k, v, h, ~m, None, gate, d ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["left", "holes", "sparse", "one"])
+@pytest.mark.parametrize("b,tq,h,d", [(1, 5, 1, 64), (2, 130, 2, 128), (1, 257, 80, 64)])
+def test_contexts_of_many_tiles(b, tq, h, d, kind):
+    """More key tiles than one pass over the list of a sample's tiles takes at a time, also
+    when a cluster's CTAs share them, and with most of them empty."""
+    tk = 9000
+    g, q, k, v, gate = inputs(tq, b, tq, tk, h, d, torch.bfloat16)
+    m = mask_of(kind, g, b, tk)
+    check(ltx_nn.cross_attention(q, k, v, h, mask=m, gate_logits=gate), q, k, v, h, ~m, None, gate, d ** -0.5)
+
+
+def test_layouts_that_are_no_row_major_view():
+    """Expanded (shared) keys, a single row with odd strides, batch-first slices: all taken."""
+    b, tq, tk, h, d = 3, 5, 40, 2, 64
+    g, q, k, v, _ = inputs(5, b, tq, tk, h, d, torch.bfloat16)
+    m = mask_of("right", g, b, tk)
+    shared = k[:1].expand(b, tk, h * d)
+    row = v[:1, :1].expand(1, tk, h * d).expand(b, tk, h * d)
+    want = ltx_nn.cross_attention(q.contiguous(), shared.contiguous(), row.contiguous(), h, mask=m)
+    assert torch.equal(ltx_nn.cross_attention(q, shared, row, h, mask=m), want)
+    qt = q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    assert torch.equal(ltx_nn.cross_attention(qt, shared, row, h, mask=m), want)
+    one = torch.randn(h * d, 1, device=DEV, dtype=torch.bfloat16).T[None]  # (1, 1, W) of strides (., 1, 1)
+    a = ltx_nn.cross_attention(one, k[:1], v[:1], h, mask=m[:1])
+    assert torch.equal(a, ltx_nn.cross_attention(one.clone(memory_format=torch.contiguous_format), k[:1], v[:1], h,
+                                                 mask=m[:1]))
