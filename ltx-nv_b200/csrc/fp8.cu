@@ -362,11 +362,14 @@ template <> LTX_DEVICE void st4v<float>(float* p, const float (&v)[4]) {
 // Epilogue of W (1, 4 or 16) accumulators, columns [col, col + W) of row `row` (sample sb, token
 // st), in fp32 and rounded once on the store: acc + bias, then the activation, residual +
 // gate * (acc + bias), or + row_vec on marked rows. W > 1 needs every vector aligned there.
-template <typename T, int W>
+template <typename T, int W, int STRIDE = 1>
 LTX_DEVICE void fp8_epilogue(const Epi<T>& e, T* __restrict__ crow, int64_t row, int64_t sb, int64_t st, int col,
-                             float (&v)[W]) {
-  auto load = [](const T* p, float (&x)[W]) {
-    if constexpr (W == 16)
+                             float (&v)[W], int N = 0) {
+  auto load = [&](const T* p, float (&x)[W]) {
+    if constexpr (STRIDE > 1) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[i] = col + i * STRIDE < N ? ld_elem<T>(p + i * STRIDE) : 0.f;
+    } else if constexpr (W == 16)
       ld16v<T>(p, x);
     else if constexpr (W == 4)
       ld4v<T>(p, x);
@@ -407,7 +410,11 @@ LTX_DEVICE void fp8_epilogue(const Epi<T>& e, T* __restrict__ crow, int64_t row,
 #pragma unroll
     for (int i = 0; i < W; ++i) v[i] += a[i];
   }
-  if constexpr (W == 16)
+  if constexpr (STRIDE > 1) {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (col + i * STRIDE < N) st_elem<T>(crow + col + i * STRIDE, v[i]);
+  } else if constexpr (W == 16)
     st16v<T>(crow + col, v);
   else if constexpr (W == 4)
     st4v<T>(crow + col, v);
@@ -464,54 +471,65 @@ struct Fp8TileCfg {
   static_assert(128 * LD_PART * 4 <= RING, "the partial tile reuses the operand ring");
 };
 
-// Rows rank, rank + SPLIT, .. of the tile whose SPLIT fp32 partials lie at `base` in the
-// cluster's CTAs: added in rank order, epilogue, store. One warp per row, so that a part's
-// row is one contiguous 512-byte read, and 8 / SPLIT rows at a time, so that 8 reads are in
-// flight (with a lane per row the reads of 128 rows and 8 parts took 20 us).
-template <typename T, int SPLIT>
-LTX_DEVICE void fp8_add_parts(const Epi<T>& epi, bool vec, T* __restrict__ C, int64_t ldc, int m0, int n0, int rows,
-                              int cols, int rank, uint32_t base) {
+// The rows rank, rank + SPLIT, .. of the tile whose SPLIT fp32 partials lie in the cluster's
+// CTAs are added in rank order into this CTA's own part (at `own`, shared address `base`).
+// One warp per row, so that a part's row is one contiguous 512-byte read, and 8 / SPLIT rows at
+// a time, so that 8 reads are in flight (with a lane per row the reads of 128 rows and 8
+// parts took 20 us).
+template <int SPLIT>
+LTX_DEVICE void fp8_add_parts(float* own, uint32_t base, int rows, int rank) {
   constexpr int U = 8 / SPLIT;
   const int lane = lane_id();
   uint32_t part[SPLIT];
 #pragma unroll
-  for (int p = 0; p < SPLIT; ++p) part[p] = (SPLIT > 1 ? mapa_shared(base, uint32_t(p)) : base) + (vec ? 16u : 4u) * lane;
+  for (int p = 0; p < SPLIT; ++p) part[p] = mapa_shared(base, uint32_t(p)) + 16u * lane;
   for (int r0 = warp_id() * SPLIT * U + rank; r0 < rows; r0 += 6 * SPLIT * U) {
     float4 x[U][SPLIT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = min(r0 + u * SPLIT, rows - 1);
+      const int r = r0 + u * SPLIT < rows ? r0 + u * SPLIT : r0;
       const uint32_t at = uint32_t(r * Fp8TileCfg::LD_PART) * 4u;
 #pragma unroll
-      for (int p = 0; p < SPLIT; ++p)
-        x[u][p] = vec ? ld_cluster_f4(part[p] + at)
-                      : make_float4(ld_cluster_f1(part[p] + at), ld_cluster_f1(part[p] + at + 128),
-                                    ld_cluster_f1(part[p] + at + 256), ld_cluster_f1(part[p] + at + 384));
+      for (int p = 0; p < SPLIT; ++p) x[u][p] = ld_cluster_f4(part[p] + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * SPLIT;
-      if (r >= rows) break;
-      float v[4] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w};
+      if (r0 + u * SPLIT >= rows) break;
 #pragma unroll
       for (int p = 1; p < SPLIT; ++p) {
-        v[0] += x[u][p].x;
-        v[1] += x[u][p].y;
-        v[2] += x[u][p].z;
-        v[3] += x[u][p].w;
+        x[u][0].x += x[u][p].x;
+        x[u][0].y += x[u][p].y;
+        x[u][0].z += x[u][p].z;
+        x[u][0].w += x[u][p].w;
       }
-      const int64_t m = int64_t(m0) + r;
-      const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
-      if (vec && lane * 4 + 4 <= cols) {
-        fp8_epilogue<T, 4>(epi, C + m * ldc, m, sb, st, n0 + lane * 4, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = vec ? lane * 4 + j : lane + 32 * j;
-          float w[1] = {v[j]};
-          if (c < cols) fp8_epilogue<T, 1>(epi, C + m * ldc, m, sb, st, n0 + c, w);
-        }
-      }
+      reinterpret_cast<float4*>(own + (r0 + u * SPLIT) * Fp8TileCfg::LD_PART)[lane] = x[u][0];
+    }
+  }
+}
+
+// Epilogue and store of the rows rank, rank + split, .. of a tile in shared memory, a warp per
+// row (the row that fp8_add_parts gave the same lanes of some warp: the caller has
+// synchronised). Lanes take four neighbouring columns, or, where those cannot be stored
+// together, columns 32 apart. The loop is kept small: with the epilogue inlined per element
+// and eight rows at a time its code ran from memory (1001 x 1371 x 1037: 25 us against 11.5).
+template <typename T>
+LTX_DEVICE void fp8_store_rows(const Epi<T>& epi, bool vec, T* __restrict__ C, int64_t ldc, int m0, int n0, int rows,
+                               int cols, int rank, int split, const float* part) {
+  const int lane = lane_id(), N = n0 + cols;
+  vec = vec && cols % 4 == 0;
+#pragma unroll 1
+  for (int r = warp_id() * split + rank; r < rows; r += 6 * split) {
+    const float* row = part + r * Fp8TileCfg::LD_PART;
+    const int64_t m = int64_t(m0) + r;
+    const int64_t sb = int64_t(int(m) / int(epi.rows_per_batch)), st = m - sb * epi.rows_per_batch;
+    if (vec) {
+      if (lane * 4 >= cols) continue;
+      const float4 x = reinterpret_cast<const float4*>(row)[lane];
+      float v[4] = {x.x, x.y, x.z, x.w};
+      fp8_epilogue<T, 4>(epi, C + m * ldc, m, sb, st, n0 + lane * 4, v);
+    } else {
+      float v[4] = {row[lane], row[lane + 32], row[lane + 64], row[lane + 96]};
+      fp8_epilogue<T, 4, 32>(epi, C + m * ldc, m, sb, st, n0 + lane, v, N);
     }
   }
 }
@@ -653,14 +671,15 @@ __global__ void __launch_bounds__(192, 2)
     else
       __syncthreads();
     const int rows = min(128, M - m0), cols = min(128, N - n0);
-    const uint32_t base = smem_u32(smem);
+    float* part = reinterpret_cast<float*>(smem);
     switch (split) {
-      case 1: fp8_add_parts<T, 1>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
-      case 2: fp8_add_parts<T, 2>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
-      case 4: fp8_add_parts<T, 4>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
-      default: fp8_add_parts<T, 8>(epi, vec, C, ldc, m0, n0, rows, cols, rank, base); break;
+      case 1: break;
+      case 2: fp8_add_parts<2>(part, smem_u32(smem), rows, rank); break;
+      case 4: fp8_add_parts<4>(part, smem_u32(smem), rows, rank); break;
+      default: fp8_add_parts<8>(part, smem_u32(smem), rows, rank); break;
     }
-    if (split > 1) cluster_sync_all();  // no CTA leaves while another reads its partial tile
+    if (split > 1) cluster_sync_all();  // sums are in place, and no CTA reads another's part any more
+    fp8_store_rows<T>(epi, vec, C, ldc, m0, n0, rows, cols, rank, split, part);
   }
   tc_fence_before();
   __syncthreads();
