@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
       for (int i = 0; i < 4; ++i) t[i] = f2_fma(v[i + 4], v[i + 4], f2_mul(v[i], v[i]));
       // one Newton step on the approximate root: within an ulp
       const float a = fmaf(row_sum(total(t)), inv_d, eps), y = rsqrtf(a);
-      const float rstd = a > 0.f && a < __int_as_float(0x7f800000) ? y * fmaf(-0.5f * a * y, y, 1.5f) : y;
+      const float rstd = a > 0.f && a < __int_as_float(0x7f800000) ? fmaf(0.5f * y, fmaf(-a * y, y, 1.f), y) : y;
       const uint64_t r2 = f2_pack(rstd, rstd);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = f2_mul(v[i], r2);
