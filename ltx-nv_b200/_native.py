@@ -591,24 +591,36 @@ def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
 class Fp8Rows:
     """A (..., cols) tensor in 8-bit floating point with a power-of-two scale per row and
     block of 128 columns (the 8-bit rows of include/ltxb200.h). `shape` is the tensor's,
-    `data` its (rows, cols) float8_e4m3fn view whose row stride is a multiple of 16, `scales`
-    the packed scale words; both are owned by this object and reused by every call that is
-    given it."""
+    `data` its (rows, cols) float8_e4m3fn view whose row stride `ld` is a multiple of 16,
+    `scales` the packed scale words; both are views of one buffer that this object owns and
+    every call that is given it reuses."""
 
-    __slots__ = ("data", "scales", "rows", "cols", "shape")
+    __slots__ = ("buf", "rows", "cols", "ld", "shape", "scale_bytes")
 
     def __init__(self, *shape: int, device: torch.device | str):
         *lead, cols = shape
         rows = math.prod(lead)
-        ld = (cols + 15) // 16 * 16
-        data = torch.empty(rows, ld, dtype=torch.float8_e4m3fn, device=device)
-        self.data = data if ld == cols else data[:, :cols]
-        self.scales = torch.empty((rows + 255) // 256 * 256 * ((cols + 511) // 512), dtype=torch.int32, device=device)
         self.rows, self.cols, self.shape = rows, cols, tuple(shape)
+        self.ld = (cols + 15) // 16 * 16
+        self.scale_bytes = (rows + 255) // 256 * 256 * ((cols + 511) // 512) * 4  # a multiple of 1024: data stays aligned
+        self.buf = torch.empty(self.scale_bytes + rows * self.ld, dtype=torch.uint8, device=device)
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self.buf[self.scale_bytes:].view(torch.float8_e4m3fn).view(self.rows, self.ld)[:, :self.cols]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.buf[:self.scale_bytes].view(torch.int32)
+
+    def operand(self) -> tuple[int, int, int]:
+        """(address of the data, its row stride, address of the scale words)."""
+        p = self.buf.data_ptr()
+        return p + self.scale_bytes, self.ld, p
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return self.buf.device
 
     @classmethod
     def from_parts(cls, data: torch.Tensor, scales: torch.Tensor) -> "Fp8Rows":
@@ -630,16 +642,15 @@ class Fp8Rows:
         out = cls(rows, cols, device=data.device)
         out.data.copy_(data)
         s = scales.contiguous()
-        _on(data, "ltx_fp8_pack_scales", s.data_ptr(), s.shape[1], rows, cols, out.scales.data_ptr())
+        _on(data, "ltx_fp8_pack_scales", s.data_ptr(), s.shape[1], rows, cols, out.operand()[2])
         return out
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values in `dtype` (float32 or bfloat16; exact in both)."""
-        out = torch.empty(self.shape, dtype=dtype, device=self.data.device)
+        out = torch.empty(self.shape, dtype=dtype, device=self.buf.device)
         dt = _dt(out)
         if out.numel():
-            _on(out, "ltx_dequantize_fp8", self.data.data_ptr(), self.data.stride(0), self.scales.data_ptr(), self.rows,
-                self.cols, out.data_ptr(), self.cols, dt)
+            _on(out, "ltx_dequantize_fp8", *self.operand(), self.rows, self.cols, out.data_ptr(), self.cols, dt)
         return out
 
 
@@ -649,8 +660,7 @@ def quantize_fp8(x: torch.Tensor, shape: tuple[int, ...] | None = None) -> Fp8Ro
     _same_device(x)
     out = Fp8Rows(*(shape or x.shape), device=x.device)
     if x.numel():
-        _on(x, "ltx_quantize_fp8", x.data_ptr(), ld, x.shape[0], x.shape[1], out.data.data_ptr(), out.data.stride(0),
-            out.scales.data_ptr(), dt)
+        _on(x, "ltx_quantize_fp8", x.data_ptr(), ld, x.shape[0], x.shape[1], *out.operand(), dt)
     return out
 
 
@@ -662,8 +672,7 @@ def norm_modulate_fp8(x: torch.Tensor, rows_per_batch: int, kind: int, eps: floa
     rows, d = x.shape
     out = Fp8Rows(*(shape or x.shape), device=x.device)
     if x.numel():
-        _on(x, "ltx_norm_modulate_fp8", x.data_ptr(), ld, out.data.data_ptr(), out.data.stride(0),
-            out.scales.data_ptr(), rows, rows_per_batch, d, kind, eps, ctypes.byref(mod) if mod is not None else None, dt)
+        _on(x, "ltx_norm_modulate_fp8", x.data_ptr(), ld, *out.operand(), rows, rows_per_batch, d, kind, eps, ctypes.byref(mod) if mod is not None else None, dt)
     return out
 
 
@@ -673,10 +682,9 @@ def linear_fp8(a: Fp8Rows, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = N
     if a.cols != w.cols or c.shape[-1] != w.rows or c.numel() != a.rows * w.rows:
         raise ValueError(f"shape mismatch a{a.shape} w{w.shape} c{tuple(c.shape)}")
     dt, ld = _dt(c), (w.rows if c.is_contiguous() else _ld(c))
-    _same_device(c, a.data, w.data)
+    _same_device(c, a.buf, w.buf)
     if c.numel():
-        _on(c, "ltx_linear_fp8", a.data.data_ptr(), a.data.stride(0), a.scales.data_ptr(), w.data.data_ptr(),
-            w.data.stride(0), w.scales.data_ptr(), c.data_ptr(), ld, a.rows, w.rows, a.cols,
+        _on(c, "ltx_linear_fp8", *a.operand(), *w.operand(), c.data_ptr(), ld, a.rows, w.rows, a.cols,
             ctypes.byref(epi) if epi is not None else None, dt,
             label=f"linear_fp8 M={a.rows} N={w.rows} K={a.cols}" if _profile is not None else None)
 
@@ -694,14 +702,13 @@ def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilo
     if k != w.cols or c.shape[-1] != w.rows or c.numel() != m * w.rows:
         raise ValueError(f"shape mismatch x{tuple(x.shape)} w{w.shape} c{tuple(c.shape)}")
     xdt, ldx, dt, ld = _dt(x), _ld(x), _dt(c), (w.rows if c.is_contiguous() else _ld(c))
-    _same_device(x, c, w.data)
+    _same_device(x, c, w.buf)
     if not c.numel():
         return
     n = load_library().ltx_quantize_linear_fp8_workspace_bytes(m, k)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _on(x, "ltx_quantize_linear_fp8", x.data_ptr(), ldx, xdt, w.data.data_ptr(), w.data.stride(0), w.scales.data_ptr(),
-        c.data_ptr(), ld, m, w.rows, k, ctypes.byref(epi) if epi is not None else None,
-        ws.data_ptr() if n else None, n, dt,
+    _on(x, "ltx_quantize_linear_fp8", x.data_ptr(), ldx, xdt, *w.operand(), c.data_ptr(), ld, m, w.rows, k,
+        ctypes.byref(epi) if epi is not None else None, ws.data_ptr() if n else None, n, dt,
         label=f"quantize_linear_fp8 M={m} N={w.rows} K={k}" if _profile is not None else None)
 
 

@@ -192,7 +192,8 @@ _NORM_KINDS = {"rms": nat.LTX_NORM_RMS, "layer": nat.LTX_NORM_LAYER, "none": nat
 def norm_modulate_fp8(x: torch.Tensor, scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
                       kind: str = "rms", eps: float = 1e-6) -> Fp8Rows:
     """norm(x) * (1 + scale) + shift of x (B, T, D) as 8-bit rows, the operand of linear_fp8:
-    fp32 arithmetic and one rounding. scale and shift (B, D) or (B, T, D) in x's type; kind "rms", "layer" or "none"; D a multiple of 8."""
+    fp32 arithmetic and one rounding. scale and shift (B, D) or (B, T, D) in x's type; kind
+    "rms", "layer" or "none"; D a multiple of 8."""
     if kind not in _NORM_KINDS:
         raise ValueError(f"kind must be one of {sorted(_NORM_KINDS)}, got {kind!r}")
     if x.dim() != 3:

@@ -8,6 +8,7 @@ import torch
 
 import _native as nat
 import fp8_reference as ref
+import ltx_dit
 import ltx_nn
 
 INVALID, UNSUPPORTED = 1, 3
@@ -81,6 +82,49 @@ def test_linear_epilogue_refusals(lib, fields, msg):
         setattr(e, k, v)
     st = lib.ltx_linear_fp8(P, 256, P, P, 256, P, P, 64, 4, 64, 256, ctypes.byref(e), 1, None)
     assert st == INVALID and msg in lib.ltx_last_error(), lib.ltx_last_error()
+
+
+@pytest.mark.parametrize("change,msg", [
+    ({"x": None}, b"non-NULL"), ({"C": None}, b"non-NULL"), ({"xdt": 2}, b"x_dtype"), ({"dtype": 2}, b"dtype must"),
+    ({"K": 0}, b"positive"), ({"ldx": 255}, b"ldx"), ({"ldc": 63}, b"ldc"), ({"x": P + 1}, b"aligned"),
+    ({"C": P + 1}, b"aligned"), ({"ldw": 250}, b"multiple of 16"), ({"W": P + 8}, b"16-byte"), ({"M": 1 << 31}, b"out of range"),
+    ({"M": 9, "ws": None}, b"workspace"), ({"M": 9, "ws": P + 4}, b"workspace"), ({"M": 9, "bytes": 9 * 256}, b"workspace")])
+def test_quantize_linear_refusals(lib, change, msg):
+    a = {"x": P, "ldx": 256, "xdt": 1, "W": P, "ldw": 256, "Ws": P, "C": P, "ldc": 64, "M": 4, "N": 64, "K": 256,
+         "epi": None, "ws": P, "bytes": 1 << 20, "dtype": 1, "stream": None} | change
+    assert lib.ltx_quantize_linear_fp8(*a.values()) == INVALID
+    assert msg in lib.ltx_last_error(), lib.ltx_last_error()
+
+
+def test_quantize_linear_workspace(lib):
+    """Nothing for up to eight rows, else the 8-bit rows of x."""
+    f = lib.ltx_quantize_linear_fp8_workspace_bytes
+    assert f(0, 256) == f(8, 256) == f(-1, 5) == 0
+    assert f(9, 1037) == 9 * 1040 + lib.ltx_fp8_scale_bytes(9, 1037)
+    assert f(8, 1 << 20) == (8 << 20) + lib.ltx_fp8_scale_bytes(8, 1 << 20)  # too wide for shared memory
+
+
+def test_rows_are_views_of_one_buffer():
+    r = nat.Fp8Rows(3, 100, 1037, device="cpu")
+    assert r.shape == (3, 100, 1037) and (r.rows, r.cols, r.ld) == (300, 1037, 1040)
+    assert tuple(r.data.shape) == (300, 1037) and r.data.stride() == (1040, 1) and r.data.dtype == torch.float8_e4m3fn
+    data, ld, scales = r.operand()
+    assert (data, ld, scales) == (r.data.data_ptr(), 1040, r.scales.data_ptr()) and (data - scales) % 16 == 0
+    assert r.scales.numel() == 512 * 3 and r.buf.numel() == 300 * 1040 + 512 * 3 * 4
+    assert nat.Fp8Rows(0, 64, device="cpu").data.shape == (0, 64) and nat.Fp8Rows(5, 0, device="cpu").data.shape == (5, 0)
+
+
+def test_masks_of_a_guidance_batch():
+    cat = ltx_dit._cat_masks
+    a = torch.arange(6)[None] < 4
+    assert cat([None, None], 6) is None
+    assert torch.equal(cat([a, None], 6), torch.stack([a[0], torch.ones(6, dtype=torch.bool)]))
+    add = torch.where(a[0], 0.0, -1e4)
+    assert torch.equal(cat([None, add, add.reshape(1, 1, 1, 6)], 6), torch.stack([torch.zeros(6), add, add]))
+    with pytest.raises(TypeError, match="one type"):
+        cat([a, add], 6)
+    with pytest.raises(RuntimeError):
+        cat([a, None], 7)
 
 
 @pytest.mark.parametrize("change,status", [
