@@ -430,6 +430,10 @@ struct MaUnit {
   uint32_t marked[2];
   uint32_t pad2[2];
 };
+// A row with a finite score has a sum of weights of at least 2^-8 (m_ref is at most the
+// taken from weighs 1, and m_ref only rises with the next such key); one of -inf scores alone
+// has the remainders of the cubic, 36 * 19 * 2^-149 a tile. Below kMaDeadRow there is no weight.
+constexpr float kMaDeadRow = 0x1p-100f;
 constexpr int kMaUnits = 4;  // units the producer may be ahead
 
 LTX_DEVICE void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -794,21 +798,24 @@ __global__ void __launch_bounds__(384, 1)
           sv[e + 3] = bb.w == -INFINITY ? -INFINITY : fmaf(sv[e + 3], P.scale_log2, bb.w);
         }
       }
+      // The maximum keeps a NaN score, and as m_ref carries it into every weight of the row:
+      // the cubic below would lose it, and only some keys take the cubic.
       float m8[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) m8[e] = sv[e];
 #pragma unroll
       for (int e = 8; e < 120; e += 16)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
+        for (int j = 0; j < 8; ++j) m8[j] = fmax3_nan(m8[j], sv[e + j], sv[e + 8 + j]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m8[j] = fmaxf(m8[j], sv[120 + j]);
-      const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+      for (int j = 0; j < 8; ++j) m8[j] = fmax3_nan(m8[j], sv[120 + j], sv[120 + j]);
+      const float mx =
+          fmax3_nan(fmax3_nan(m8[0], m8[1], m8[2]), fmax3_nan(m8[3], m8[4], m8[5]), fmax3_nan(m8[6], m8[7], m8[7]));
       const float m_cand = MARKED ? mx : mx * P.scale_log2;
-      const bool need = first || (m_cand > m_ref + 8.f);
+      const bool need = first || !(m_cand <= m_ref + 8.f);
       float alpha = 1.f;
       if (need) {
-        const float m_new = fmaxf(m_ref, m_cand);
+        const float m_new = fmax3_nan(m_ref, m_cand, m_cand);
         alpha = first || m_new == -INFINITY ? 0.f : ex2_approx(m_ref - m_new);
         m_ref = m_new;
       }
@@ -912,13 +919,19 @@ __global__ void __launch_bounds__(384, 1)
       const int qi = P.q0(unit) + qt * 128 + row;
       const bool live = qi < P.Tq;
       const int64_t orow = int64_t(b) * P.Tq + qi;
-      float f = l_run == 0.f ? 0.f : 1.f / l_run;
+      const bool dead = l_run < kMaDeadRow;
+      const bool any_dead = __any_sync(0xffffffffu, dead);
+      float f = dead ? 0.f : 1.f / l_run;
       if (P.gate != nullptr && live) f *= 2.f / (1.f + __expf(-__bfloat162float(P.gate[orow * P.ld_gate + h])));
       __nv_bfloat16* op = P.O + orow * P.ldo + int64_t(h) * D;
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t rr[32];
         tmem_read32(o_tmem + uint32_t(c0), rr);
+        if (any_dead) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) rr[e] = dead ? 0u : rr[e];
+        }
         if (live) {
 #pragma unroll
           for (int e8 = 0; e8 < 32; e8 += 8) {
@@ -937,7 +950,7 @@ __global__ void __launch_bounds__(384, 1)
       float* part = reinterpret_cast<float*>(smem);
       float* lse = part + 256 * Cfg::LD_PART;
       const int r = qt * 128 + row;
-      const bool some = have && l_run != 0.f;
+      const bool some = have && !(l_run < kMaDeadRow);
       if (have) {
         const float inv = some ? 1.f / l_run : 0.f;
 #pragma unroll

@@ -590,16 +590,28 @@ LTX_DEVICE float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// The same, NaN if any of them is.
+LTX_DEVICE float fmax3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // 2^x on the FMA / integer pipes, to take load off the special-function unit:
 // Cody-Waite range reduction x = n + f, n = round(x) (by the 1.5*2^23 shifter trick),
 // f in [-1/2, 1/2], 2^f by a cubic whose coefficients were fitted to minimise the
 // relative error on that interval (max relative error 7.6e-5), and 2^n added into the
-// exponent field. Valid for -126 <= x <= 127; callers pass finite x <= 8.
+// exponent field. Valid for -126 <= x <= 127; callers pass x <= 8 (a NaN is lost: callers
+// that want it kept look at the row's maximum). Smaller x are raised to kEx2Floor, whose
+// cubic is the first value from 1 upwards (1 + 19 * 2^-23), so that the exponent field
+// drops to zero and what is left, 19 * 2^-149, rounds to zero in bf16: -inf weighs nothing.
+// A floor of -126 left 2^-126, which times a value of 2^127 is 2. Between the floor and -126
+// the result is below 2^-126 and not accurate.
 // The shifted sum t = x + 1.5*2^23 has the bit pattern 0x4B400000 + n, and
 // 0x4B400000 << 23 wraps to 0 in 32 bits, so (bits(t) << 23) == (n << 23).
+constexpr float kEx2Floor = -0x1.fbffe4p+6f;  // -127 + 14 * 2^-17
 LTX_DEVICE float ex2_poly(float x) {
-  x = fmaxf(x, -126.f);
+  x = fmaxf(x, kEx2Floor);
   const float t = x + 12582912.f;
   const float f = x - (t - 12582912.f);
   const float p = fmaf(fmaf(fmaf(0.0551708005f, f, 0.242609262f), f, 0.693260968f), f, 0.999928176f);
@@ -608,8 +620,8 @@ LTX_DEVICE float ex2_poly(float x) {
 
 // The same for two values with packed fp32x2 arithmetic.
 LTX_DEVICE void ex2_poly2(float x0, float x1, float& y0, float& y1) {
-  x0 = fmaxf(x0, -126.f);
-  x1 = fmaxf(x1, -126.f);
+  x0 = fmaxf(x0, kEx2Floor);
+  x1 = fmaxf(x1, kEx2Floor);
   const uint64_t shifter = f2_pack(12582912.f, 12582912.f);
   const uint64_t x = f2_pack(x0, x1);
   const uint64_t t = f2_add(x, shifter);

@@ -274,3 +274,79 @@ def test_layouts_that_are_no_row_major_view():
     a = ltx_nn.cross_attention(one, k[:1], v[:1], h, mask=m[:1])
     assert torch.equal(a, ltx_nn.cross_attention(one.clone(memory_format=torch.contiguous_format), k[:1], v[:1], h,
                                                  mask=m[:1]))
+
+
+# -------------------------------------------- NaN and -inf scores of keys that take part
+
+
+@pytest.mark.parametrize("masked", ["none", "first", "last"])
+@pytest.mark.parametrize("tq,tk", [(40, 256), (300, 200), (20, 640)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_at_every_kept_key_reaches_its_head(d, tq, tk, masked):
+    """Wherever in a tile of 128 keys the NaN lies, and whether the tile holds a left-out key
+    (`masked`) or not, every query of that head gets NaN, and the other head keeps its bits."""
+    b, h = 1, 2
+    g, q, k, v, _ = inputs(11, b, tq, tk, h, d, torch.bfloat16)
+    m = torch.ones(b, tk, dtype=torch.bool, device=DEV)
+    if masked != "none":
+        m[0, 0 if masked == "first" else tk - 1] = False
+    clean = ltx_nn.cross_attention(q, k, v, h, mask=m)
+    keys = [i for i in (*range(128), *range(128, tk, 37)) if m[0, i]]
+    for c0 in (0, d):  # the NaN's head
+        lost = []
+        for key in keys:
+            k2 = k.clone()
+            k2[0, key, c0 + key % d] = math.nan
+            got = ltx_nn.cross_attention(q, k2, v, h, mask=m)
+            other = slice(d - c0, 2 * d - c0)
+            if not (torch.isnan(got[..., c0:c0 + d]).all() and torch.equal(got[..., other], clean[..., other])):
+                lost.append(key)
+        assert not lost, lost
+    q2 = q.clone()
+    q2[0, 7, 3] = math.nan
+    got = ltx_nn.cross_attention(q2, k, v, h, mask=m)
+    assert torch.isnan(got[0, 7, :d]).all()
+    got[0, 7, :d] = clean[0, 7, :d]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("tq,tk", [(1, 256), (40, 128), (300, 384), (20, 640)])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
+def test_rows_of_minus_infinite_scores_are_zero(dtype, d, tq, tk, masked):
+    b, h = 2, 2
+    g, q, k, v, gate = inputs(12, b, tq, tk, h, d, dtype)
+    m = torch.ones(b, tk, dtype=torch.bool, device=DEV)
+    if masked:
+        m[:, 5] = False
+    want = ltx_nn.cross_attention(q, k, v, h, mask=m, gate_logits=gate)
+    q2, k2 = q.clone(), k.clone()
+    q2[1, :, 0] = q[1, :, 0].abs() + 1
+    k2[1, :, 0] = -math.inf  # sample 1, head 0: every score is -inf
+    got = ltx_nn.cross_attention(q2, k2, v, h, mask=m, gate_logits=gate)
+    assert (got[1, :, :d] == 0).all(), got[1, :, :d].abs().max()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, :, d:], want[1, :, d:])
+
+
+@pytest.mark.parametrize("low", [-math.inf, -4e4, -2000.0])
+@pytest.mark.parametrize("tq,tk", [(40, 256), (300, 128), (20, 640)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_far_below_the_maximum_weigh_nothing(d, tq, tk, low):
+    """Kept keys whose scores are -inf, or hundreds below the row's largest, have weights below
+    exp(-200) = 2^-288: with values of 2^120 they add less than 2^-160, so the result is that
+    of the other keys."""
+    b, h = 1, 2
+    g, q, k, v, _ = inputs(13, b, tq, tk, h, d, torch.bfloat16)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    q[..., ::d] = 2.0
+    k[..., ::d] = 0.0
+    m = torch.ones(b, tk, dtype=torch.bool, device=DEV)
+    low_keys = torch.arange(tk, device=DEV) % 3 == 1
+    left_out = low_keys[None].expand(b, tk)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, low_keys] = 0.0
+    k2[:, low_keys, ::d] = low
+    v2[:, low_keys] = 2.0 ** 120
+    got = ltx_nn.cross_attention(q, k2, v2, h, mask=m, scale=0.1)
+    k[:, low_keys], v[:, low_keys] = 0.0, 0.0
+    check(got, q, k, v, h, left_out, None, None, 0.1)
