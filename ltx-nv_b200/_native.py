@@ -345,8 +345,10 @@ def _ld(t: torch.Tensor) -> int:
 
 def modulation(table: torch.Tensor | None, mod: torch.Tensor | None, *, shift: tuple[int, int] | None,
                scale: tuple[int, int] | None, mod_ld_batch: int = 0, mod_ld_tok: int = 0) -> Modulation:
-    """Describe shift/scale vectors table[t_off:] + mod[b, t, m_off:] (element offsets)."""
+    """Describe shift/scale vectors table[t_off:] + mod[b, t, m_off:] (element offsets). The
+    struct holds addresses; the object keeps the tensors behind them alive."""
     m = Modulation()
+    m.tensors = (table, mod)
     m.table = _ptr(table)
     m.mod = _ptr(mod)
     m.mod_ld_batch = mod_ld_batch
@@ -458,7 +460,10 @@ def timestep_embedding(t: torch.Tensor, scale: float, dim: int, max_period: floa
 def epilogue(kind: int = EPI_NONE, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
              gate: Modulation | None = None, rows_per_batch: int = 1, row_mask: torch.Tensor | None = None,
              row_vec: torch.Tensor | None = None, silu_input: bool = False) -> Epilogue:
+    """The epilogue of a linear layer. The struct holds addresses; the object keeps the tensors
+    behind them alive, so that a copy made for this call outlives its launch."""
     e = Epilogue()
+    e.tensors = (bias, residual, gate, row_mask, row_vec)
     e.kind = kind
     e.bias = _ptr(bias)
     if residual is not None:

@@ -2,6 +2,7 @@
 no GPU is touched (every check comes before the first CUDA call)."""
 
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -211,3 +212,36 @@ def test_masks_refused():
         ltx_nn.cross_attention(q, k.float(), k, 2, mask=ones)
     with pytest.raises(ValueError, match="out must"):
         call(ones, out=torch.zeros(2, 5, 128))
+
+
+@pytest.mark.parametrize("bias", ["strided", "expanded"])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_copies_made_for_an_epilogue_live_until_the_launch(monkeypatch, bias, quantised):
+    """The epilogue holds addresses: a vector that had to be copied must still exist when the
+    launch reads it (its memory could be given to the call's own workspace otherwise)."""
+    copies, calls = [], []
+    contiguous = torch.Tensor.contiguous
+
+    def copying(t, *a, **kw):
+        r = contiguous(t, *a, **kw)
+        if r is not t:
+            copies.append((r.data_ptr(), weakref.ref(r)))
+        return r
+
+    def launch(x, w, c, epi):
+        alive = {p for p, ref_ in copies if ref_() is not None}
+        calls.append(epi.bias in alive and epi.gate.mod in alive)
+
+    monkeypatch.setattr(torch.Tensor, "contiguous", copying)
+    monkeypatch.setattr(nat, "quantize_linear_fp8", launch)
+    monkeypatch.setattr(nat, "linear_fp8", launch)
+    monkeypatch.setattr(nat, "_ptr", lambda t: t.data_ptr() if t is not None else None)
+    x = torch.zeros(2, 5, 256, dtype=torch.bfloat16)
+    if quantised:
+        x = nat.Fp8Rows(2, 5, 256, device="cpu")
+    wide = torch.zeros(64, 2, dtype=torch.bfloat16)
+    b = wide[:, 0] if bias == "strided" else wide[:1, 0].expand(64)
+    gate = torch.zeros(2, 128, dtype=torch.bfloat16)[:, ::2]
+    ltx_nn.linear_fp8(x, nat.Fp8Rows(64, 256, device="cpu"), b, residual=torch.zeros(2, 5, 64, dtype=torch.bfloat16),
+                      gate=gate)
+    assert len(copies) == 2 and calls == [True]

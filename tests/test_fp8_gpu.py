@@ -340,3 +340,17 @@ def test_linear_fp8_on_another_stream_and_captured():
         buf.copy_(new)
         graph.replay()
         assert torch.equal(out, step(new))
+
+
+@pytest.mark.parametrize("m", [2, 9, 252])
+def test_linear_fp8_takes_a_bias_of_any_stride(m):
+    g = gen(m)
+    n, k = 640, 512
+    x, w = randn(g, m, k), nat.quantize_fp8(randn(g, n, k, std=0.05))
+    buf = randn(g, n, 3)
+    for bias in (buf[:, 0], buf[:1, 1].expand(n)):
+        want = ltx_nn.linear_fp8(x, w, bias.clone(memory_format=torch.contiguous_format).contiguous())
+        for _ in range(3):
+            assert torch.equal(ltx_nn.linear_fp8(x, w, bias), want)
+            assert torch.equal(ltx_nn.linear_fp8(nat.quantize_fp8(x), w, bias), ltx_nn.linear_fp8(
+                nat.quantize_fp8(x), w, bias.contiguous()))
