@@ -256,7 +256,10 @@ int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, const void*
 /* ltx_quantize_fp8 of x (M, K) in x_dtype, then ltx_linear_fp8, in one call: up to eight rows
  * in one launch that quantises them while it streams W, more through the workspace (device
  * memory, 16-byte aligned, ltx_quantize_linear_fp8_workspace_bytes(M, K) bytes, 0 when none is
- * needed; no initialisation; calls that may run concurrently need one each). */
+ * needed; no initialisation; calls that may run concurrently need one each). C may overlap x
+ * (x, C and the residual may be one matrix): x is then quantised by a launch of its own for any
+ * M, and the workspace must hold M * (K rounded up to 16) + ltx_fp8_scale_bytes(M, K) bytes, or
+ * the call is rejected. */
 size_t ltx_quantize_linear_fp8_workspace_bytes(int64_t M, int64_t K);
 int ltx_quantize_linear_fp8(const void* x, int64_t ldx, int x_dtype, const void* W, int64_t ldw, const void* w_scales,
                             void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, const ltx_epilogue* epi,

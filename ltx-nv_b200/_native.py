@@ -702,7 +702,7 @@ def fp8_force_pair(pair: int) -> None:
 def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = None) -> None:
     """c = epilogue(quantize_fp8(x) @ w.T (+ bias)); x (M, K) float32 or bfloat16 with unit
     column stride, c (M, N) a row-major view in the epilogue's type, or any contiguous (..., N)
-    tensor of M rows."""
+    tensor of M rows; c may overlap x."""
     m, k = x.shape
     if k != w.cols or c.shape[-1] != w.rows or c.numel() != m * w.rows:
         raise ValueError(f"shape mismatch x{tuple(x.shape)} w{w.shape} c{tuple(c.shape)}")
@@ -710,7 +710,12 @@ def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilo
     _same_device(x, c, w.buf)
     if not c.numel():
         return
-    n = load_library().ltx_quantize_linear_fp8_workspace_bytes(m, k)
+    lib = load_library()
+    n = lib.ltx_quantize_linear_fp8_workspace_bytes(m, k)
+    if n == 0:  # none is needed, unless the result may overwrite x
+        px, pc = x.data_ptr(), c.data_ptr()
+        if px < pc + ((m - 1) * ld + w.rows) * c.element_size() and pc < px + ((m - 1) * ldx + k) * x.element_size():
+            n = m * ((k + 15) // 16 * 16) + lib.ltx_fp8_scale_bytes(m, k)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     _on(x, "ltx_quantize_linear_fp8", x.data_ptr(), ldx, xdt, *w.operand(), c.data_ptr(), ld, m, w.rows, k,
         ctypes.byref(epi) if epi is not None else None, ws.data_ptr() if n else None, n, dt,

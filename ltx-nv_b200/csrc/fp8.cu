@@ -1341,10 +1341,20 @@ extern "C" int ltx_linear_fp8(const void* A, int64_t lda, const void* a_scales, 
 
 // Workspace of ltx_quantize_linear_fp8: the quantised rows' data, then their scales.
 static size_t quantized_data_bytes(int64_t M, int64_t K) { return size_t(M) * size_t((K + 15) / 16 * 16); }
+static size_t quantized_bytes(int64_t M, int64_t K) { return quantized_data_bytes(M, K) + ltx_fp8_scale_bytes(M, K); }
 
 extern "C" size_t ltx_quantize_linear_fp8_workspace_bytes(int64_t M, int64_t K) {
   if (M <= 0 || K <= 0 || fp8_use_rows(M, K)) return 0;
-  return (quantized_data_bytes(M, K) + 15) / 16 * 16 + ltx_fp8_scale_bytes(M, K);
+  return quantized_bytes(M, K);
+}
+
+// Whether any of M rows of `a` (na bytes, lda between rows) shares a byte with one of `b`.
+static bool rows_overlap(const void* a, int64_t lda, int64_t na, const void* b, int64_t ldb, int64_t nb, int64_t M) {
+  const intptr_t pa = reinterpret_cast<intptr_t>(a), pb = reinterpret_cast<intptr_t>(b);
+  for (int64_t i = 0; i < M; ++i)
+    for (int64_t j = 0; j < M; ++j)
+      if (pa + i * lda < pb + j * ldb + nb && pb + j * ldb < pa + i * lda + na) return true;
+  return false;
 }
 
 extern "C" int ltx_quantize_linear_fp8(const void* x, int64_t ldx, int x_dtype, const void* W, int64_t ldw,
@@ -1363,12 +1373,17 @@ extern "C" int ltx_quantize_linear_fp8(const void* x, int64_t ldx, int x_dtype, 
   LTX_REQUIRE(reinterpret_cast<uintptr_t>(x) % (x_dtype == LTX_F32 ? 4 : 2) == 0, "x is not aligned to its type");
   LTX_REQUIRE(reinterpret_cast<uintptr_t>(C) % (dtype == LTX_F32 ? 4 : 2) == 0, "C is not aligned to its type");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (!fp8_use_rows(M, K)) {
+  // Every CTA of the streaming kernel quantises x for itself, at its own time: the result must
+  // not overwrite x before the last of them has.
+  const int64_t xs = x_dtype == LTX_F32 ? 4 : 2, cs = dtype == LTX_F32 ? 4 : 2;
+  if (!fp8_use_rows(M, K) || rows_overlap(x, ldx * xs, K * xs, C, ldc * cs, N * cs, M)) {
     LTX_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
-                    workspace_bytes >= ltx_quantize_linear_fp8_workspace_bytes(M, K),
-                "the workspace must be 16-byte aligned and hold ltx_quantize_linear_fp8_workspace_bytes(M, K) bytes");
+                    workspace_bytes >= quantized_bytes(M, K),
+                "the workspace must be 16-byte aligned and hold the 8-bit rows of x: "
+                "ltx_quantize_linear_fp8_workspace_bytes(M, K) bytes, and where C overlaps x M * (K rounded up to 16) "
+                "+ ltx_fp8_scale_bytes(M, K) for any M");
     const int64_t ldq = (K + 15) / 16 * 16;
-    void* scales = static_cast<char*>(workspace) + (quantized_data_bytes(M, K) + 15) / 16 * 16;
+    void* scales = static_cast<char*>(workspace) + quantized_data_bytes(M, K);
     bool unused;  // the epilogue is checked before the first launch
     if (dtype == LTX_F32)
       make_epi_any<float>(epi, N, unused);

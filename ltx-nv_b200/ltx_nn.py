@@ -218,7 +218,7 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
     (norm_modulate_fp8). weight: (N, K) Fp8Rows. The result is (..., N) in `dtype` (default:
     x's type; for 8-bit rows the residual's, or bfloat16). gate: (B, N) per sample or (B, T,
     N) per token of a (B, T, N) result; bias, residual and gate are in `dtype`. out may be the
-    residual itself."""
+    residual itself, and x too."""
     if not isinstance(weight, Fp8Rows):
         raise TypeError("weight must be Fp8Rows (quantize_fp8 or Fp8Rows.from_parts)")
     if activation not in _ACTIVATIONS:

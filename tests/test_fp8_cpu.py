@@ -245,3 +245,32 @@ def test_copies_made_for_an_epilogue_live_until_the_launch(monkeypatch, bias, qu
     ltx_nn.linear_fp8(x, nat.Fp8Rows(64, 256, device="cpu"), b, residual=torch.zeros(2, 5, 64, dtype=torch.bfloat16),
                       gate=gate)
     assert len(copies) == 2 and calls == [True]
+
+
+def test_quantize_linear_in_place_needs_the_workspace(lib):
+    """Where C shares a byte with x, the rows are quantised before anything is stored."""
+    a = {"x": P, "ldx": 256, "xdt": 1, "W": P, "ldw": 256, "Ws": P, "C": P, "ldc": 256, "M": 4, "N": 256, "K": 256,
+         "epi": None, "ws": None, "bytes": 0, "dtype": 1, "stream": None}
+    need = 4 * 256 + lib.ltx_fp8_scale_bytes(4, 256)
+    for change in ({}, {"C": P + 2 * (3 * 256 + 255)}, {"C": P + 2 * 255, "ldx": 512, "ldc": 512}, {"M": 1},
+                   {"x": P + 2 * (3 * 256 + 255)}, {"ws": P, "bytes": need - 1}, {"ws": P + 4, "bytes": need},
+                   {"xdt": 0, "dtype": 0, "C": P + 1020}):
+        assert lib.ltx_quantize_linear_fp8(*(a | change).values()) == INVALID
+        assert b"overlaps x" in lib.ltx_last_error(), change
+
+
+def test_quantize_linear_passes_a_workspace_when_in_place(monkeypatch):
+    sizes = []
+    monkeypatch.setattr(nat, "_same_device", lambda *a: None)
+    monkeypatch.setattr(nat, "_on", lambda t, name, *args, **kw: sizes.append(args[13]))
+    w = nat.Fp8Rows(256, 256, device="cpu")
+    buf = torch.zeros(8, 512, dtype=torch.bfloat16)
+    nat.quantize_linear_fp8(buf[:4, :256], w, torch.zeros(4, 256, dtype=torch.bfloat16))
+    nat.quantize_linear_fp8(buf[:4, :256], w, buf[4:, :256])
+    assert sizes == [0, 0]
+    x = torch.zeros(4, 256, dtype=torch.bfloat16)
+    nat.quantize_linear_fp8(x, w, x)
+    ltx_nn.linear_fp8(x, w, out=x)
+    nat.quantize_linear_fp8(buf[:4, :256], w, buf[3:7, :256])
+    need = 4 * 256 + nat.load_library().ltx_fp8_scale_bytes(4, 256)
+    assert sizes[2:] == [need] * 3

@@ -354,3 +354,27 @@ def test_linear_fp8_takes_a_bias_of_any_stride(m):
             assert torch.equal(ltx_nn.linear_fp8(x, w, bias), want)
             assert torch.equal(ltx_nn.linear_fp8(nat.quantize_fp8(x), w, bias), ltx_nn.linear_fp8(
                 nat.quantize_fp8(x), w, bias.contiguous()))
+
+
+@pytest.mark.parametrize("m", [1, 2, 8, 9, 200])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_fp8_in_place(m, dtype):
+    """x, residual and out may be one tensor: the result is that of the rows quantised first."""
+    g = gen(m)
+    n = 2048
+    x, w, bias = randn(g, 1, m, n, dtype=dtype), nat.quantize_fp8(randn(g, n, n, std=0.02)), randn(g, n, dtype=dtype)
+    want = ltx_nn.linear_fp8(ltx_nn.quantize_fp8(x), w, bias, residual=x)
+    plain = ltx_nn.linear_fp8(ltx_nn.quantize_fp8(x), w, bias, dtype=dtype)
+    for _ in range(5):
+        buf = x.clone()
+        assert ltx_nn.linear_fp8(buf, w, bias, residual=buf, out=buf) is buf
+        assert torch.equal(buf, want)
+        buf = x.clone()
+        ltx_nn.linear_fp8(buf, w, bias, out=buf)
+        assert torch.equal(buf, plain)
+    # rows of one buffer that interleave without sharing a byte
+    wide = torch.zeros(m, 2 * n, dtype=dtype, device=DEV)
+    wide[:, :n] = x[0]
+    nat.quantize_linear_fp8(wide[:, :n], w, wide[:, n:], nat.epilogue(bias=bias))
+    assert torch.equal(wide[:, :n], x[0])
+    assert torch.equal(wide[:, n:], ltx_nn.linear_fp8(x, w, bias)[0])
