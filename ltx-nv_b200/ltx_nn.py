@@ -152,6 +152,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     """x (..., K) float32 or bfloat16 -> its 8-bit rows: e4m3 values with a power-of-two scale
     per 128 columns. Weights (N, K) are quantised with it once."""
+    if x.shape[-1] == 0:
+        raise ValueError("x has no columns")
     return nat.quantize_fp8(_row_major(x), x.shape)
 
 
@@ -232,6 +234,8 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
         dtype = x.dtype if isinstance(x, torch.Tensor) else residual.dtype if residual is not None else torch.bfloat16
     if x.shape[-1] != weight.cols or len(weight.shape) != 2:
         raise ValueError(f"x has {x.shape[-1]} columns, the weight is {weight.shape}")
+    if weight.cols == 0:
+        raise ValueError("the weight has no columns")
     lead = x.shape[:-1]
     shape = (*lead, n)
     dev = x.device
@@ -260,7 +264,7 @@ def linear_fp8(x, weight: Fp8Rows, bias: torch.Tensor | None = None, *, activati
                        residual=residual2 if residual is not None else None, gate=mod, rows_per_batch=rpb)
     if isinstance(x, Fp8Rows):
         nat.linear_fp8(x, weight, out, epi)
-    elif weight.cols:
+    else:
         nat.quantize_linear_fp8(_row_major(x), weight, out, epi)
     return out
 

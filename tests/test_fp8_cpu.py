@@ -274,3 +274,16 @@ def test_quantize_linear_passes_a_workspace_when_in_place(monkeypatch):
     nat.quantize_linear_fp8(buf[:4, :256], w, buf[3:7, :256])
     need = 4 * 256 + nat.load_library().ltx_fp8_scale_bytes(4, 256)
     assert sizes[2:] == [need] * 3
+
+
+def test_weights_without_columns_are_refused():
+    """An empty reduction has no blocks and no 8-bit form: refused for both kinds of x, before
+    a result is allocated."""
+    w = nat.Fp8Rows(5, 0, device="cpu")
+    for x in (torch.zeros(3, 0), nat.Fp8Rows(3, 0, device="cpu")):
+        with pytest.raises(ValueError, match="no columns"):
+            ltx_nn.linear_fp8(x, w)
+        with pytest.raises(ValueError, match="no columns"):
+            ltx_nn.linear_fp8(x, w, residual=torch.zeros(3, 5), dtype=torch.float32)
+    with pytest.raises(ValueError, match="no columns"):
+        ltx_nn.quantize_fp8(torch.zeros(3, 0))
