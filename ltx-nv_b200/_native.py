@@ -659,11 +659,15 @@ class Fp8Rows:
         return out
 
 
-def quantize_fp8(x: torch.Tensor, shape: tuple[int, ...] | None = None) -> Fp8Rows:
-    """x (rows, cols) float32 or bfloat16, unit column stride -> 8-bit rows (of `shape`)."""
+def quantize_fp8(x: torch.Tensor, shape: tuple[int, ...] | None = None, out: Fp8Rows | None = None) -> Fp8Rows:
+    """x (rows, cols) float32 or bfloat16, unit column stride -> 8-bit rows (of `shape`), new
+    ones or `out`."""
     dt, ld = _dt(x), _ld(x)
-    _same_device(x)
-    out = Fp8Rows(*(shape or x.shape), device=x.device)
+    _same_device(x, out.buf if out is not None else None)
+    if out is None:
+        out = Fp8Rows(*(shape or x.shape), device=x.device)
+    elif (out.rows, out.cols) != tuple(x.shape):
+        raise ValueError(f"out holds {out.rows} x {out.cols} values, x is {tuple(x.shape)}")
     if x.numel():
         _on(x, "ltx_quantize_fp8", x.data_ptr(), ld, x.shape[0], x.shape[1], *out.operand(), dt)
     return out

@@ -258,8 +258,11 @@ class LTXModel(torch.nn.Module):
         the parameter), every norm in front of a product writes 8-bit rows, other operands
         are quantised by the product's call. The projection of a text context that is cached
         over the denoise steps, the adaLN layers, the patchify and output projections and
-        all of attention stay in the model's type. Call it again after loading other
-        weights. NativeStep keeps running the parameters as they are."""
+        all of attention stay in the model's type. The 8-bit forms follow load_state_dict,
+        moves and in-place operations (ltx_nn.Fp8Module); after writes that torch does not
+        count (through .data), or before replaying a graph that was captured earlier, call
+        this again: it writes the same 8-bit rows. NativeStep keeps running the parameters
+        as they are."""
         for blk in self.blocks:
             for attn in (blk.attn1, blk.audio_attn1):
                 attn.quantize_fp8(("self",))
@@ -430,7 +433,7 @@ class LTXModel(torch.nn.Module):
                        st.mod(table, st.tmod, 6, 7) if cfg.cross_attention_adaln else None, "q" in attn2.fp8)
         wq, bq = attn2.packed_q()
         qg = torch.empty(rows, wq.shape[0], device=h.device, dtype=h.dtype)
-        project(hq, wq, attn2.fp8.get("q"), qg, nat.epilogue(bias=bq))
+        project(hq, wq, attn2.weight8("q", wq), qg, nat.epilogue(bias=bq))
         attn2._norm_rope(qg[:, :inner], st.T, attn2.q_norm.weight, None)
         ctx = st.context
         if cfg.cross_attention_adaln:
@@ -443,7 +446,7 @@ class LTXModel(torch.nn.Module):
                                            mod_ld_batch=st.prompt_mod.shape[-1]), fp8)
             wkv, bkv = attn2.packed_kv()
             kv = torch.empty(ctx.shape[0], wkv.shape[0], device=h.device, dtype=h.dtype)
-            project(enc, wkv, attn2.fp8.get("kv"), kv, nat.epilogue(bias=bkv))
+            project(enc, wkv, attn2.weight8("kv", wkv), kv, nat.epilogue(bias=bkv))
             attn2._norm_rope(kv[:, :inner], st.S, attn2.k_norm.weight, None)
         else:
             kv = self._text_kv(attn2, ctx, st.S, st.context_src if st.context_src is not None else ctx)
@@ -502,11 +505,11 @@ class LTXModel(torch.nn.Module):
         gated = self.cfg.gated_attention
         wq, bq = attn.packed_q()
         qg = torch.empty(q_in.shape[0], wq.shape[0], device=wq.device, dtype=wq.dtype)
-        project(q_in, wq, attn.fp8.get("q"), qg, nat.epilogue(bias=bq))
+        project(q_in, wq, attn.weight8("q", wq), qg, nat.epilogue(bias=bq))
         attn._norm_rope(qg[:, :inner], q_st.T, attn.q_norm.weight, q_pe)
         wkv, bkv = attn.packed_kv()
         kv = torch.empty(kv_in.shape[0], wkv.shape[0], device=wq.device, dtype=wq.dtype)
-        project(kv_in, wkv, attn.fp8.get("kv"), kv, nat.epilogue(bias=bkv))
+        project(kv_in, wkv, attn.weight8("kv", wkv), kv, nat.epilogue(bias=bkv))
         attn._norm_rope(kv[:, :inner], kv_st.T, attn.k_norm.weight, k_pe)
         if self._sp is not None and kv_st.name == "video":
             # video-to-audio under sequence parallelism: the video keys are sharded over

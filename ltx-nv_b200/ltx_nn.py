@@ -149,12 +149,15 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
 # ---------------------------------------------------------------------------------------
 
 
-def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+def quantize_fp8(x: torch.Tensor, out: Fp8Rows | None = None) -> Fp8Rows:
     """x (..., K) float32 or bfloat16 -> its 8-bit rows: e4m3 values with a power-of-two scale
-    per 128 columns. Weights (N, K) are quantised with it once."""
+    per 128 columns. Weights (N, K) are quantised with it once. out: rows of x's shape to
+    write to instead of new ones."""
     if x.shape[-1] == 0:
         raise ValueError("x has no columns")
-    return nat.quantize_fp8(_row_major(x), x.shape)
+    if out is not None and out.shape != tuple(x.shape):
+        raise ValueError(f"out is {out.shape}, x is {tuple(x.shape)}")
+    return nat.quantize_fp8(_row_major(x), x.shape, out)
 
 
 def _modulation(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None):
@@ -484,23 +487,94 @@ def _pack(mod: torch.nn.Module, names: list[str], attr: str) -> tuple[torch.Tens
     rows = sum(s.weight.shape[0] for s in subs)
     pad = (-rows) % 8  # keep the packed output's row stride a multiple of 8 elements
     ref = subs[0].weight
-    w = torch.zeros(rows + pad, ref.shape[1], device=ref.device, dtype=ref.dtype)
-    b = torch.zeros(rows + pad, device=ref.device, dtype=ref.dtype)
-    torch.cat([s.weight.detach() for s in subs], dim=0, out=w[:rows])
-    torch.cat([s.bias.detach() for s in subs], dim=0, out=b[:rows])
-    row = 0
-    for s in subs:
-        n = s.weight.shape[0]
-        s.weight.data = w[row:row + n]
-        s.bias.data = b[row:row + n]
-        row += n
+    with torch.inference_mode(False):  # the parameters stay ordinary tensors, whose writes torch counts
+        w = torch.zeros(rows + pad, ref.shape[1], device=ref.device, dtype=ref.dtype)
+        b = torch.zeros(rows + pad, device=ref.device, dtype=ref.dtype)
+        torch.cat([s.weight.detach() for s in subs], dim=0, out=w[:rows])
+        torch.cat([s.bias.detach() for s in subs], dim=0, out=b[:rows])
+        row = 0
+        for s in subs:
+            n = s.weight.shape[0]
+            s.weight.data = w[row:row + n]
+            s.bias.data = b[row:row + n]
+            row += n
     setattr(mod, key, (w, b, [s.weight.data_ptr() for s in subs]))
     return w, b
 
 
-class Attention(torch.nn.Module):
+def _version(t: torch.Tensor) -> int:
+    """torch's count of in-place writes; -1 for inference tensors, which have none."""
+    return -1 if t.is_inference() else t._version
+
+
+def _requantize_fp8(module: "Fp8Module", _incompatible_keys) -> None:
+    for name in list(module.fp8):
+        module.weight8(name, module._fp8_weight(name), loaded=True)
+
+
+class Fp8Module(torch.nn.Module):
+    """A module that may hold 8-bit forms of its weights beside the parameters: fp8, name ->
+    Fp8Rows, which weight8 gives to the products. They follow the parameters: load_state_dict
+    quantises the new ones, and weight8 those that have been moved, replaced or written by an
+    in-place operation since (not what torch does not count: writes through .data, or to
+    inference tensors; quantise again after those). The same rows are written, so captured
+    graphs that read them follow too."""
+
+    FP8_PARTS: dict[str, tuple[str, ...]] = {}  # name -> the Linear sub-modules it packs
+
+    def __init__(self):
+        super().__init__()
+        self.fp8: dict[str, Fp8Rows] = {}
+        self._fp8_stamps: dict[str, tuple] = {}
+        self.register_load_state_dict_post_hook(_requantize_fp8)
+
+    def _fp8_weight(self, name: str) -> torch.Tensor:
+        """The parameter or packed weight that fp8[name] is the 8-bit form of."""
+        return getattr(self, self.FP8_PARTS[name][0]).weight
+
+    def _fp8_stamp(self, name: str, weight: torch.Tensor) -> tuple:
+        parts = [self._modules.get(n) for n in self.FP8_PARTS[name]]
+        return (weight.data_ptr(), _version(weight), *[_version(m.weight) for m in parts if m is not None])
+
+    def _quantize_weight(self, name: str, weight: torch.Tensor) -> None:
+        rows = self.fp8.get(name)
+        if rows is not None and (name not in self._fp8_stamps or rows.shape != tuple(weight.shape)
+                                 or rows.device != weight.device):
+            rows = None  # the caller's, or of another weight
+        stamp = self._fp8_stamp(name, weight)
+        self.fp8[name] = quantize_fp8(weight.detach(), rows)
+        self._fp8_stamps[name] = stamp
+
+    def _quantize_weights(self, names: tuple[str, ...]) -> None:
+        """8-bit forms of these weights, and of no others, as they are now."""
+        for name in set(self.fp8) - set(names):
+            del self.fp8[name]
+            self._fp8_stamps.pop(name, None)
+        for name in names:
+            self._quantize_weight(name, self._fp8_weight(name))
+
+    def weight8(self, name: str, weight: torch.Tensor, loaded: bool = False) -> Fp8Rows | None:
+        """The 8-bit form of `weight`, in step with it; None if it has none. Rows that a caller
+        put into fp8 are taken as they are. loaded: the weight has just been written."""
+        rows = self.fp8.get(name)
+        if rows is None or name not in self._fp8_stamps:
+            return rows
+        if loaded and not weight.is_cuda:
+            self._fp8_stamps[name] = ()  # quantised when it is back on the GPU and used
+        elif loaded or self._fp8_stamps[name] != self._fp8_stamp(name, weight):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the weights have changed since they were quantised: quantise them, or run the "
+                                   "module once, before the capture")
+            self._quantize_weight(name, weight)
+        return self.fp8[name]
+
+
+class Attention(Fp8Module):
     """ltx_nn.py:166-236: gated multi-head attention with q/k RMSNorm over the inner
     dim and split RoPE. Same parameters and forward signature as the reference."""
+
+    FP8_PARTS = {"self": ("to_q", "to_k", "to_v", "to_gate_logits"), "q": ("to_q", "to_gate_logits"),
+                 "kv": ("to_k", "to_v"), "out": ("to_out",)}
 
     def __init__(self, query_dim: int, context_dim: int | None = None, heads: int = 8, dim_head: int = 64,
                  norm_eps: float = 1e-6, apply_gated_attention: bool = False):
@@ -517,14 +591,15 @@ class Attention(torch.nn.Module):
         self.to_v = torch.nn.Linear(context_dim, inner, bias=True)
         self.to_gate_logits = torch.nn.Linear(query_dim, heads, bias=True) if apply_gated_attention else None
         self.to_out = torch.nn.Linear(inner, query_dim, bias=True)
-        self.fp8: dict[str, Fp8Rows] = {}  # 8-bit weights by packing, after quantize_fp8
 
     def quantize_fp8(self, packings: tuple[str, ...]) -> None:
         """8-bit forms of the named packed weights ("self", or "q" and "kv") and of to_out,
         used from now on; the parameters stay as they are."""
+        self._quantize_weights((*packings, "out"))
+
+    def _fp8_weight(self, name: str) -> torch.Tensor:
         packed = {"self": self.packed_self, "q": self.packed_q, "kv": self.packed_kv}
-        self.fp8 = {name: quantize_fp8(packed[name]()[0]) for name in packings}
-        self.fp8["out"] = quantize_fp8(self.to_out.weight.detach())
+        return packed[name]()[0] if name in packed else self.to_out.weight
 
     # packed weights -----------------------------------------------------------------
     def packed_self(self):
@@ -547,7 +622,7 @@ class Attention(torch.nn.Module):
         inner = self.heads * self.dim_head
         w, b = self.packed_self()
         qkv = torch.empty(x2.shape[0], w.shape[0], device=w.device, dtype=w.dtype)
-        project(x2, w, self.fp8.get("self"), qkv, nat.epilogue(bias=b))
+        project(x2, w, self.weight8("self", w), qkv, nat.epilogue(bias=b))
         if not normalize:
             return qkv
         if k_pe is None:
@@ -589,7 +664,8 @@ class Attention(torch.nn.Module):
         return o
 
     def project_out(self, o: torch.Tensor, out: torch.Tensor, epi: nat.Epilogue) -> None:
-        project(o, self.to_out.weight, self.fp8.get("out"), out, epi)
+        weight = self.to_out.weight
+        project(o, weight, self.weight8("out", weight), out, epi)
 
     def forward(self, x: torch.Tensor, context: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                 pe=None, k_pe=None, perturbation_mask: torch.Tensor | None = None,
@@ -614,10 +690,10 @@ class Attention(torch.nn.Module):
             c2 = context.reshape(b * s, -1)
             wq, bq = self.packed_q()
             qg = torch.empty(b * t, wq.shape[0], device=x.device, dtype=x.dtype)
-            project(x2, wq, self.fp8.get("q"), qg, nat.epilogue(bias=bq))
+            project(x2, wq, self.weight8("q", wq), qg, nat.epilogue(bias=bq))
             wkv, bkv = self.packed_kv()
             kv = torch.empty(b * s, 2 * inner, device=x.device, dtype=x.dtype)
-            project(c2, wkv, self.fp8.get("kv"), kv, nat.epilogue(bias=bkv))
+            project(c2, wkv, self.weight8("kv", wkv), kv, nat.epilogue(bias=bkv))
             self._norm_rope(qg[:, :inner], t, self.q_norm.weight, pe_t)
             self._norm_rope(kv[:, :inner], s, self.k_norm.weight, kpe_t if kpe_t is not None else pe_t)
             o = self.attend(qg[:, :inner], kv[:, :inner], kv[:, inner:], qg[:, inner:] if gated else None, b, t, s, mask)
@@ -626,8 +702,10 @@ class Attention(torch.nn.Module):
         return out.view(b, t, -1)
 
 
-class FeedForward(torch.nn.Module):
+class FeedForward(Fp8Module):
     """ltx_nn.py:239-248: proj_out(gelu_tanh(proj_in(x)))."""
+
+    FP8_PARTS = {"in": ("proj_in",), "out": ("proj_out",)}
 
     def __init__(self, dim: int, dim_out: int | None = None, mult: int = 4, bias: bool = True):
         super().__init__()
@@ -635,17 +713,17 @@ class FeedForward(torch.nn.Module):
         inner = int(dim * mult)
         self.proj_in = torch.nn.Linear(dim, inner, bias=bias)
         self.proj_out = torch.nn.Linear(inner, dim_out, bias=bias)
-        self.fp8: dict[str, Fp8Rows] = {}  # 8-bit weights, after quantize_fp8
 
     def quantize_fp8(self) -> None:
         """8-bit forms of both weights, used from now on; the parameters stay as they are."""
-        self.fp8 = {"in": quantize_fp8(self.proj_in.weight.detach()), "out": quantize_fp8(self.proj_out.weight.detach())}
+        self._quantize_weights(("in", "out"))
 
     def run(self, x2, out: torch.Tensor, epi: nat.Epilogue) -> None:
         """out = epilogue(proj_out(gelu_tanh(proj_in(x2)))), x2 (rows, dim) or its 8-bit rows."""
         h = torch.empty(out.shape[0], self.proj_in.out_features, device=out.device, dtype=out.dtype)
-        project(x2, self.proj_in.weight, self.fp8.get("in"), h, nat.epilogue(nat.EPI_GELU_TANH, bias=self.proj_in.bias))
-        project(h, self.proj_out.weight, self.fp8.get("out"), out, epi)
+        w_in, w_out = self.proj_in.weight, self.proj_out.weight
+        project(x2, w_in, self.weight8("in", w_in), h, nat.epilogue(nat.EPI_GELU_TANH, bias=self.proj_in.bias))
+        project(h, w_out, self.weight8("out", w_out), out, epi)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         b, t, d = x.shape

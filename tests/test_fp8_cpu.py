@@ -287,3 +287,85 @@ def test_weights_without_columns_are_refused():
             ltx_nn.linear_fp8(x, w, residual=torch.zeros(3, 5), dtype=torch.float32)
     with pytest.raises(ValueError, match="no columns"):
         ltx_nn.quantize_fp8(torch.zeros(3, 0))
+
+
+class _FakeQuantiser:
+    """Stands in for the quantiser: rows on the CPU that remember the weight's values."""
+
+    def __init__(self, monkeypatch):
+        self.seen = {}
+        monkeypatch.setattr(ltx_nn, "quantize_fp8", self)
+
+    def __call__(self, x, out=None):
+        rows = out if out is not None else nat.Fp8Rows(*x.shape, device="cpu")
+        self.seen[id(rows)] = (rows, x.clone())
+        return rows
+
+    def holds(self, module, name):
+        rows = module.weight8(name, module._fp8_weight(name))
+        return torch.equal(self.seen[id(rows)][1], module._fp8_weight(name))
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_quantised_weights_follow_the_parameters(monkeypatch, inference):
+    fake = _FakeQuantiser(monkeypatch)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    attn = ltx_nn.Attention(64, 128, heads=1, dim_head=64, apply_gated_attention=True)
+    ff = ltx_nn.FeedForward(64)
+    with torch.inference_mode(inference):
+        attn.quantize_fp8(("q", "kv"))
+        ff.quantize_fp8()
+    kept = {(id(m), n): m.fp8[n] for m in (attn, ff) for n in m.fp8}
+
+    def step(change):
+        for m in (attn, ff):
+            change(m)
+        for m in (attn, ff):
+            for n in m.fp8:
+                assert fake.holds(m, n), (type(m).__name__, n)
+                assert m.fp8[n] is kept[id(m), n]  # the same rows: captured graphs read them
+
+    step(lambda m: m.load_state_dict({k: torch.randn_like(v) for k, v in m.state_dict().items()}))
+    step(lambda m: m.load_state_dict({k: torch.randn_like(v) for k, v in m.state_dict().items()}, assign=True))
+
+    def merge(m):
+        with torch.no_grad():
+            for p in m.parameters():
+                p.add_(0.5)
+
+    step(merge)
+    with torch.inference_mode():
+        step(merge)
+    step(lambda m: m.to(torch.bfloat16))
+    def uncounted(m):
+        for p in m.parameters():
+            p.data.mul_(2)
+        m.quantize_fp8(("q", "kv")) if m is attn else m.quantize_fp8()
+
+    step(uncounted)
+    count = len(fake.seen)
+    assert all(m.weight8(n, m._fp8_weight(n)) is m.fp8[n] for m in (attn, ff) for n in m.fp8) and len(fake.seen) == count
+    assert attn.weight8("self", attn.to_q.weight) is None
+    # rows that a caller put there are the caller's
+    own = nat.Fp8Rows(64, 64, device="cpu")
+    attn.fp8["own"] = own
+    assert attn.weight8("own", attn.to_q.weight) is own
+    del attn.fp8["own"]
+    # not in the middle of a capture, which would quantise at every replay
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    merge(ff)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        ff.weight8("in", ff.proj_in.weight)
+
+
+def test_quantise_into_rows(monkeypatch):
+    with pytest.raises(ValueError, match="out is"):
+        ltx_nn.quantize_fp8(torch.zeros(3, 64), nat.Fp8Rows(4, 64, device="cpu"))
+    monkeypatch.setattr(nat, "_same_device", lambda *a: None)
+    with pytest.raises(ValueError, match="out holds"):
+        nat.quantize_fp8(torch.zeros(3, 64), out=nat.Fp8Rows(4, 64, device="cpu"))
+    calls = []
+    monkeypatch.setattr(nat, "_on", lambda t, name, *args, **kw: calls.append(args))
+    rows = nat.Fp8Rows(3, 64, device="cpu")
+    assert ltx_nn.quantize_fp8(torch.zeros(3, 64), rows) is rows
+    assert calls[0][4:7] == rows.operand()

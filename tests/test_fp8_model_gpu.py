@@ -227,3 +227,105 @@ def test_connector_without_registers_against_the_oracle(dtype):
     got, out_mask = conn(x.to(DEV), mask.to(DEV))
     assert rel_l2(got, want) < (1e-2 if dtype == torch.bfloat16 else 1e-4)
     assert torch.equal(out_mask.cpu(), mask)
+
+
+# ----------------------------------------------------------------- weights that change
+
+
+def _modules():
+    torch.manual_seed(21)
+    attn = ltx_nn.Attention(256, 192, heads=4, dim_head=64, apply_gated_attention=True).to(DEV, torch.bfloat16)
+    ff = ltx_nn.FeedForward(256).to(DEV, torch.bfloat16)
+    attn.quantize_fp8(("q", "kv"))
+    ff.quantize_fp8()
+    return attn, ff
+
+
+def test_quantised_modules_follow_their_weights():
+    """After load_state_dict, in-place updates and moves the products use what the parameters
+    hold now: the bits of a module that was quantised with them."""
+    attn, ff = _modules()
+    x = torch.randn(2, 70, 256, device=DEV, dtype=torch.bfloat16)
+    ctx = torch.randn(2, 50, 192, device=DEV, dtype=torch.bfloat16)
+
+    def outputs(a, f):
+        with torch.inference_mode():
+            return a(x, ctx), f(x)
+
+    def fresh():
+        a = ltx_nn.Attention(256, 192, heads=4, dim_head=64, apply_gated_attention=True).to(DEV, torch.bfloat16)
+        f = ltx_nn.FeedForward(256).to(DEV, torch.bfloat16)
+        a.load_state_dict(attn.state_dict())
+        f.load_state_dict(ff.state_dict())
+        a.quantize_fp8(("q", "kv"))
+        f.quantize_fp8()
+        return outputs(a, f)
+
+    def merge():
+        with torch.no_grad():
+            for m in (attn, ff):
+                for name, p in m.named_parameters():
+                    if name.startswith(("to_", "proj_")):
+                        p.add_(torch.randn_like(p) * 0.02)
+
+    def load():
+        for m in (attn, ff):
+            m.load_state_dict({k: v + torch.randn_like(v) * 0.02 for k, v in m.state_dict().items()})
+
+    def move():
+        for m in (attn, ff):
+            m.to(torch.float32)
+            merge()
+            m.to(torch.bfloat16)
+
+    old = outputs(attn, ff)
+    for change in (load, merge, move):
+        change()
+        new = outputs(attn, ff)
+        for a, b, c in zip(new, fresh(), old):
+            assert torch.equal(a, b) and not torch.equal(a, c), change.__name__
+        old = new
+
+
+def test_captured_products_follow_loaded_weights():
+    """A graph reads the 8-bit rows by address: loading weights, and quantising again, write the
+    same rows."""
+    attn, ff = _modules()
+    x = torch.randn(2, 70, 256, device=DEV, dtype=torch.bfloat16)
+    ctx = torch.randn(2, 50, 192, device=DEV, dtype=torch.bfloat16)
+
+    def step():
+        return ff(attn(x, ctx))
+
+    with torch.inference_mode():
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for again in (False, True):
+            for m in (attn, ff):
+                if again:
+                    for p in m.parameters():
+                        p.data.mul_(0.9)
+                else:
+                    m.load_state_dict({k: v + torch.randn_like(v) * 0.02 for k, v in m.state_dict().items()})
+            if again:
+                attn.quantize_fp8(("q", "kv"))
+                ff.quantize_fp8()
+            graph.replay()
+            assert torch.equal(out, step())
+
+
+def test_quantised_model_with_other_weights_loaded():
+    cfg = small_cfg()
+    model, _ = philox_model(cfg, 31, host_copy=False)
+    other, _ = philox_model(cfg, 32, host_copy=False)
+    model.quantize_fp8()
+    video = video_inputs(cfg, torch.bfloat16)
+    first, _ = model(video, None)
+    model.load_state_dict(other.state_dict())
+    video.context = video.context.clone()  # the projection of a context is cached with it
+    got, _ = model(video, None)
+    other.quantize_fp8()
+    assert torch.equal(got, other(video, None)[0]) and not torch.equal(got, first)
