@@ -1065,10 +1065,13 @@ __global__ void __launch_bounds__(256, 2)
         const float a1 = 2 * piece + 1 < M ? sa[(2 * piece + 1) * quads * 4 + kb] : 0.f;
         const float s0 = fp8_scale((sw[j][0] >> (8 * (kb & 3))) & 255u);
         const float s1 = fp8_scale((sw[j][1] >> (8 * (kb & 3))) & 255u);
-        acc[0] = fmaf(c[0] * a0, s0, acc[0]);
-        acc[1] = fmaf(c[1] * a1, s0, acc[1]);
-        acc[2] = fmaf(c[2] * a0, s1, acc[2]);
-        acc[3] = fmaf(c[3] * a1, s1, acc[3]);
+        // The scales' product first: it is exact, and infinite or zero only where the result is
+        // above 2^110 or below 2^-124 as well. c times one scale (2^118) could leave fp32 before
+        // the other brings it back.
+        acc[0] = fmaf(c[0], a0 * s0, acc[0]);
+        acc[1] = fmaf(c[1], a1 * s0, acc[1]);
+        acc[2] = fmaf(c[2], a0 * s1, acc[2]);
+        acc[3] = fmaf(c[3], a1 * s1, acc[3]);
       }
       if (i0 + PRE < per_warp) fetch(n0, i0 + PRE);
     }

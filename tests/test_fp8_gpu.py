@@ -378,3 +378,19 @@ def test_linear_fp8_in_place(m, dtype):
     nat.quantize_linear_fp8(wide[:, :n], w, wide[:, n:], nat.epilogue(bias=bias))
     assert torch.equal(wide[:, :n], x[0])
     assert torch.equal(wide[:, n:], ltx_nn.linear_fp8(x, w, bias)[0])
+
+
+@pytest.mark.parametrize("m", [1, 3, 8, 9])
+@pytest.mark.parametrize("ex,ew", [(100, -95), (-110, 100), (118, -118), (-118, 118), (58, 60), (-58, -60),
+                                   (-63, -62)])
+def test_linear_fp8_of_huge_and_tiny_operands(m, ex, ew):
+    """Scales whose product is in range: partial products of a block that carry one operand's
+    scale alone would leave fp32."""
+    g = gen(m + ex)
+    k, n = 1000, 260
+    x = randn(g, m, k, dtype=torch.float32) * 2.0 ** ex
+    w = randn(g, n, k, dtype=torch.float32) * 2.0 ** ew
+    wq = nat.quantize_fp8(w)
+    a, b = nat.quantize_fp8(x).dequantize(torch.float32).double(), wq.dequantize(torch.float32).double()
+    got = ltx_nn.linear_fp8(x, wq).double()
+    assert ((got - a @ b.t()).abs() <= (a.abs() @ b.abs().t()) * k * 2.0 ** -23).all()
