@@ -1029,7 +1029,7 @@ __global__ void __launch_bounds__(256, 2)
       }
     }
   };
-  int n0 = blockIdx.x * 16;
+  unsigned n0 = blockIdx.x * 16;  // unsigned: the step behind the last rows may pass 2^31
   fetch(n0, 0);
   for (int i = warp; i < M * quads; i += 8) {
     const int m = i / quads, kq = i - m * quads;
@@ -1042,7 +1042,7 @@ __global__ void __launch_bounds__(256, 2)
   }
   __syncthreads();
   const int per_warp = (blocks - warp + 7) / 8;
-  for (int buf = 0; n0 < N; n0 += int(gridDim.x) * 16, buf ^= 1) {
+  for (int buf = 0; n0 < unsigned(N); n0 += gridDim.x * 16, buf ^= 1) {
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < per_warp; i0 += PRE) {
 #pragma unroll
@@ -1075,14 +1075,14 @@ __global__ void __launch_bounds__(256, 2)
       }
       if (i0 + PRE < per_warp) fetch(n0, i0 + PRE);
     }
-    const int next = n0 + int(gridDim.x) * 16;
-    if (next < N) fetch(next, 0);
+    const unsigned next = n0 + gridDim.x * 16;
+    if (next < unsigned(N)) fetch(next, 0);
     *reinterpret_cast<float2*>(&part[buf][warp][row][2 * piece]) = make_float2(acc[0], acc[1]);
     *reinterpret_cast<float2*>(&part[buf][warp][row + 8][2 * piece]) = make_float2(acc[2], acc[3]);
     __syncthreads();  // the other buffer is rewritten only behind the next one
     for (int i = threadIdx.x; i < 16 * M; i += 256) {
       const int m = i >> 4, r = i & 15;
-      if (n0 + r < N) {
+      if (n0 + r < unsigned(N)) {
         float v[1] = {0.f};
 #pragma unroll
         for (int p = 0; p < 8; ++p) v[0] += part[buf][p][r][m];

@@ -394,3 +394,23 @@ def test_linear_fp8_of_huge_and_tiny_operands(m, ex, ew):
     a, b = nat.quantize_fp8(x).dequantize(torch.float32).double(), wq.dequantize(torch.float32).double()
     got = ltx_nn.linear_fp8(x, wq).double()
     assert ((got - a @ b.t()).abs() <= (a.abs() @ b.abs().t()) * k * 2.0 ** -23).all()
+
+
+def test_linear_fp8_of_nearly_2_to_the_31_weight_rows():
+    """Row indices up to the documented limit: the step behind a CTA's last rows passes 2^31."""
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 48 GB of device memory")
+    n = 2 ** 31 - 257
+    w = nat.Fp8Rows(n, 1, device=DEV)
+    w.buf[:w.scale_bytes].fill_(127)  # every scale 1
+    w.buf[w.scale_bytes:].fill_(0x38)  # every value 1
+    marked = torch.tensor([0, 15, 4735, 4736, 2 ** 30 + 1, n - 4737, n - 4736, n - 17, n - 1], device=DEV)
+    w.buf[w.scale_bytes + marked * w.ld] = 0x40  # 2
+    x = torch.full((1, 1), 3.0, device=DEV, dtype=torch.bfloat16)
+    out = ltx_nn.linear_fp8(x, w)[0]
+    assert (out[marked] == 6).all()
+    out[marked] = 3.0
+    assert int(out.min()) == 3 and int(out.max()) == 3
+    assert nat.device_error_flags() == 0
+    del w, out
+    torch.cuda.empty_cache()
