@@ -941,6 +941,7 @@ __global__ void __launch_bounds__(384, 1)
             st8<__nv_bfloat16>(op + c0 + e8, v);
           }
         }
+        __syncwarp();  // the next read is the whole warp's
       }
     }
     if (P.split > 1) {

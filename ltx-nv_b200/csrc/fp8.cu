@@ -646,13 +646,12 @@ __global__ void __launch_bounds__(192, 2)
       for (int c0 = 0; c0 < 128 && n0 + c0 < N; c0 += 32) {
         uint32_t rr[32];
         tmem_read32(tquad + uint32_t(c0), rr);
-        if (!live) continue;
-        if (staged) {
+        if (live && staged) {
           // every MMA of this CTA has read its operands: the ring is free
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             *reinterpret_cast<uint4*>(part + c0 + j) = make_uint4(rr[j], rr[j + 1], rr[j + 2], rr[j + 3]);
-        } else {
+        } else if (live) {
 #pragma unroll
           for (int j = 0; j < 32; j += 16) {
             float v[16];
@@ -661,6 +660,7 @@ __global__ void __launch_bounds__(192, 2)
             fp8_epilogue_cols<T>(epi, true, C + m * ldc, m, sb, st, n0 + c0 + j, N, v);
           }
         }
+        __syncwarp();  // the next read is the whole warp's
       }
     }
   }
@@ -868,16 +868,16 @@ __global__ void __launch_bounds__(320, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(tover), 0));
         }
-        if (!live) continue;
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {
-          if (n0 + c0 + c < N) {
+          if (live && n0 + c0 + c < N) {
             float v[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(rr[c + e]);
             fp8_epilogue_cols<T>(epi, vec, crow, m, sb, st, n0 + c0 + c, N, v);
           }
         }
+        __syncwarp();  // the next read is the whole warp's
       }
       tc_fence_before();
       __syncwarp();
