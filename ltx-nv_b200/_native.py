@@ -652,6 +652,7 @@ class Fp8Rows:
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values in `dtype` (float32 or bfloat16; exact in both)."""
+        _same_device(self.buf)
         out = torch.empty(self.shape, dtype=dtype, device=self.buf.device)
         dt = _dt(out)
         if out.numel():

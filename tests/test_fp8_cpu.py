@@ -369,3 +369,10 @@ def test_quantise_into_rows(monkeypatch):
     rows = nat.Fp8Rows(3, 64, device="cpu")
     assert ltx_nn.quantize_fp8(torch.zeros(3, 64), rows) is rows
     assert calls[0][4:7] == rows.operand()
+
+
+def test_rows_on_the_host_are_not_given_to_a_kernel():
+    """Rows moved to the host (a pickled model, say) have addresses no kernel may read."""
+    for dtype in (torch.bfloat16, torch.float32):
+        with pytest.raises(ValueError, match="CUDA"):
+            nat.Fp8Rows(3, 64, device="cpu").dequantize(dtype)
