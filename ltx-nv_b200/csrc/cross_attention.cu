@@ -1079,6 +1079,8 @@ extern "C" int ltx_attention_masked(const void* q, int64_t ldq, const void* k, i
   LTX_REQUIRE(ld_mask == 0 || ld_mask >= Tk, "ld_mask must be 0 or hold the keys");
   LTX_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   if (gate_logits) LTX_REQUIRE(ld_gate >= heads, "ld_gate must be >= heads");
+  LTX_REQUIRE(reinterpret_cast<uintptr_t>(gate_logits) % (dtype == LTX_F32 ? 4 : 2) == 0,
+              "gate_logits is not aligned to its type");
   LTX_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldo % 8 == 0, "leading dims must be multiples of 8");
   check_vec_ptr(q, "q");
   check_vec_ptr(k, "k");

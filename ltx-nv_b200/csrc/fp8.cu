@@ -1163,6 +1163,8 @@ Epi<T> make_epi_any(const ltx_epilogue* p, int64_t N, bool& vec) {
   if (e.kind == LTX_EPI_ROW_MASK_ADD) {
     if (p->row_mask == nullptr || p->row_vec == nullptr)
       throw ApiError{LTX_ERR_INVALID, "ROW_MASK_ADD needs row_mask and row_vec"};
+    if (reinterpret_cast<uintptr_t>(p->row_mask) % 4)
+      throw ApiError{LTX_ERR_INVALID, "row_mask is not aligned to its type"};
     e.row_mask = p->row_mask;
     e.row_vec = take(p->row_vec);
   }
@@ -1247,6 +1249,7 @@ extern "C" int ltx_fp8_pack_scales(const float* s, int64_t ld, int64_t rows, int
                                    void* stream) {
   LTX_API_BEGIN
   LTX_REQUIRE(s != nullptr && scales != nullptr, "s and scales must be non-NULL");
+  LTX_REQUIRE(reinterpret_cast<uintptr_t>(s) % 4 == 0, "s is not aligned to its type");
   LTX_REQUIRE(rows > 0 && cols > 0, "rows and columns must be positive");
   LTX_REQUIRE(rows < (int64_t(1) << 31) - 256 && cols < (int64_t(1) << 31) - 512, "size out of range");
   const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block;

@@ -376,3 +376,17 @@ def test_rows_on_the_host_are_not_given_to_a_kernel():
     for dtype in (torch.bfloat16, torch.float32):
         with pytest.raises(ValueError, match="CUDA"):
             nat.Fp8Rows(3, 64, device="cpu").dequantize(dtype)
+
+
+def test_operands_that_are_not_aligned_to_their_type_are_refused(lib):
+    """Every remaining pointer that a kernel reads by element: scales, row masks, gate logits."""
+    assert lib.ltx_fp8_pack_scales(P + 2, 2, 4, 256, P, None) == INVALID
+    assert b"aligned" in lib.ltx_last_error()
+    e = nat.Epilogue()
+    e.kind, e.row_mask, e.row_vec = nat.EPI_ROW_MASK_ADD, P + 2, P
+    assert lib.ltx_linear_fp8(P, 256, P, P, 256, P, P, 64, 4, 64, 256, ctypes.byref(e), 1, None) == INVALID
+    assert b"row_mask" in lib.ltx_last_error()
+    for dtype, gate in ((0, P + 2), (1, P + 1)):
+        assert lib.ltx_attention_masked(P, 128, P, 128, P, 128, P, 128, 2, 5, 100, 2, 64, 0.125, P, 100, 0, gate, 2, dtype,
+                                        None) == INVALID
+        assert b"gate_logits" in lib.ltx_last_error()
