@@ -205,8 +205,9 @@ int ltx_attention_ws(const void* q, int64_t ldq, const void* k, int64_t ldk, con
  * LTX_MASK_BOOL bytes, 0 = the key is left out; LTX_MASK_F32 / LTX_MASK_BF16 values added to
  * the scaled scores, a key being left out at or below half of the type's lowest finite
  * value (-inf included). K and V of a left-out key do not reach the output, whatever they
- * hold. A row without keys (or whose scores are all -inf) is zero. scale > 0. bf16: head_dim
- * 64 or 128, and above four queries a sample at most 524288 keys; fp32: 32, 64 or 128. */
+ * hold. A row without keys (or whose scores are all -inf) is zero. o may be q, but must not
+ * overlap k or v. scale > 0. bf16: head_dim 64 or 128, and above four queries a sample at most
+ * 524288 keys; fp32: 32, 64 or 128. */
 typedef enum { LTX_MASK_BOOL = 0, LTX_MASK_F32 = 1, LTX_MASK_BF16 = 2 } ltx_mask_kind;
 int ltx_attention_masked(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* o,
                          int64_t ldo, int B, int64_t Tq, int64_t Tk, int heads, int head_dim, float scale,

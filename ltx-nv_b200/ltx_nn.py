@@ -102,6 +102,15 @@ def _token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x2, x2.stride(0)
 
 
+def _spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the addresses from the first to the last element of a and of b overlap."""
+    if not a.numel() or not b.numel():
+        return False
+    pa, pb = a.data_ptr(), b.data_ptr()
+    na, nb = (1 + sum([(n - 1) * st for n, st in zip(t.shape, t.stride())]) for t in (a, b))
+    return pa < pb + nb * b.element_size() and pb < pa + na * a.element_size()
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int,
                     mask: torch.Tensor | None = None, gate_logits: torch.Tensor | None = None,
                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -114,7 +123,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     to the scores, a key being left out where it is at or below half of the type's lowest
     finite value. What k and v hold at a key that is left out does not matter. A sample
     without any key gives zeros (torch's softmax would give NaN, or a mean over the padding
-    for masks of the lowest value). Without a mask this is the framework's attention."""
+    for masks of the lowest value). out may be q, but not overlap k or v. Without a mask this
+    is the framework's attention."""
     b, tq, width = q.shape
     tk = k.shape[1]
     if heads <= 0 or width % heads:
@@ -127,6 +137,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         out = torch.empty(b, tq, width, device=q.device, dtype=q.dtype)
     elif tuple(out.shape) != (b, tq, width) or not out.is_contiguous() or out.dtype != q.dtype:
         raise ValueError(f"out must be a contiguous {q.dtype} ({b}, {tq}, {width}) tensor")
+    elif _spans_overlap(out, k) or _spans_overlap(out, v):
+        raise ValueError("out must not overlap k or v, which other queries still read")
     if mask is not None:
         mask = key_mask(mask, b, tk)
     if out.numel() == 0:

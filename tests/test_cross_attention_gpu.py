@@ -350,3 +350,16 @@ def test_keys_far_below_the_maximum_weigh_nothing(d, tq, tk, low):
     got = ltx_nn.cross_attention(q, k2, v2, h, mask=m, scale=0.1)
     k[:, low_keys], v[:, low_keys] = 0.0, 0.0
     check(got, q, k, v, h, left_out, None, None, 0.1)
+
+
+@pytest.mark.parametrize("b,tq,tk,h,d,dtype", [(2, 1, 900, 4, 128, torch.bfloat16), (3, 4, 200, 3, 64, torch.bfloat16),
+                                               (1, 40, 3000, 2, 64, torch.bfloat16), (2, 600, 300, 5, 128, torch.bfloat16),
+                                               (1, 9, 300, 2, 64, torch.float32), (8, 300, 70, 9, 64, torch.float32)])
+def test_the_result_may_be_written_over_the_queries(b, tq, tk, h, d, dtype):
+    g, q, k, v, gate = inputs(15, b, tq, tk, h, d, dtype)
+    m = mask_of("holes", g, b, tk)
+    want = ltx_nn.cross_attention(q, k, v, h, mask=m, gate_logits=gate)
+    for _ in range(5):
+        buf = q.contiguous().clone()
+        assert ltx_nn.cross_attention(buf, k, v, h, mask=m, gate_logits=gate, out=buf) is buf
+        assert torch.equal(buf, want)

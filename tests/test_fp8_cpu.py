@@ -390,3 +390,19 @@ def test_operands_that_are_not_aligned_to_their_type_are_refused(lib):
         assert lib.ltx_attention_masked(P, 128, P, 128, P, 128, P, 128, 2, 5, 100, 2, 64, 0.125, P, 100, 0, gate, 2, dtype,
                                         None) == INVALID
         assert b"gate_logits" in lib.ltx_last_error()
+
+
+def test_masked_attention_refuses_to_write_over_its_keys():
+    """Blocks of queries read every key of their head, each at its own time: a result over k or
+    v would be read as keys. Over q it is fine: a query's row is read before it is written."""
+    buf = torch.zeros(3, 2, 9, 128, dtype=torch.bfloat16)
+    q, k, v = buf
+    ones = torch.ones(2, 9, dtype=torch.bool)
+    across = buf.view(-1)[200:200 + k.numel()].view(2, 9, 128)  # starts inside q, ends inside k
+    for out in (k, v, across):
+        with pytest.raises(ValueError, match="overlap"):
+            ltx_nn.cross_attention(q, k, v, 2, mask=ones, out=out)
+    with pytest.raises(ValueError, match="CUDA"):
+        ltx_nn.cross_attention(q, k, v, 2, mask=ones, out=q)
+    with pytest.raises(ValueError, match="CUDA"):
+        ltx_nn.cross_attention(q, k, v, 2, mask=ones, out=torch.empty_like(q))
