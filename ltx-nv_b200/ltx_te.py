@@ -49,13 +49,9 @@ class ConnectorBlock(torch.nn.Module):
         gated = attn.to_gate_logits is not None
         o = attn.attend(qkv[:, :inner], qkv[:, inner:2 * inner], qkv[:, 2 * inner:3 * inner],
                         qkv[:, 3 * inner:3 * inner + attn.heads] if gated else None, batch, s, s, mask)
-        nat.linear(o, attn.to_out.weight, x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn.to_out.bias, residual=x,
-                                                          rows_per_batch=s))
+        attn.project_out(o, x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=attn.to_out.bias, residual=x, rows_per_batch=s))
         nat.norm_modulate(x, h, s, nat.LTX_NORM_RMS, NORM_EPS, None)
-        f = torch.empty(x.shape[0], ff.proj_in.out_features, device=x.device, dtype=x.dtype)
-        nat.linear(h, ff.proj_in.weight, f, nat.epilogue(nat.EPI_GELU_TANH, bias=ff.proj_in.bias))
-        nat.linear(f, ff.proj_out.weight, x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=ff.proj_out.bias, residual=x,
-                                                          rows_per_batch=s))
+        ff.run(h, x, nat.epilogue(nat.EPI_GATE_RESIDUAL, bias=ff.proj_out.bias, residual=x, rows_per_batch=s))
 
     def forward(self, x: torch.Tensor, additive_mask=None, pe=None) -> torch.Tensor:
         b, s, d = x.shape

@@ -329,3 +329,22 @@ def test_quantised_model_with_other_weights_loaded():
     got, _ = model(video, None)
     other.quantize_fp8()
     assert torch.equal(got, other(video, None)[0]) and not torch.equal(got, first)
+
+
+def test_connector_block_runs_its_quantised_weights():
+    """Modules that were quantised are used so wherever they stand: four 8-bit products a block."""
+    conn = ltx_te.Embeddings1DConnector(heads=4, dim_head=64, num_layers=1, max_pos=[64], registers=0, gated=False,
+                                        ff_bias=True)
+    sd = ltx_oracle.synthetic_state_dict([(k, tuple(v.shape)) for k, v in conn.named_parameters()], 5)
+    conn.load_state_dict(sd)
+    conn = conn.to(DEV, torch.bfloat16)
+    x = torch.randn(2, 48, 256, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    want = conn.blocks[0](x)
+    conn.blocks[0].attn1.quantize_fp8(("self",))
+    conn.blocks[0].ff.quantize_fp8()
+    with nat.profile() as prof:
+        got = conn.blocks[0](x)
+    calls = prof.summary()
+    assert sum(v["launches"] for k, v in calls.items() if "linear_fp8" in k) == 4
+    assert not any(k.startswith("linear ") for k in calls)
+    assert 1e-4 < rel_l2(got, want) < 0.15
