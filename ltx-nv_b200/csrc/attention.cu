@@ -372,9 +372,11 @@ __device__ __forceinline__ void fmha_body(const CUtensorMap* tmQ_, const CUtenso
 #pragma unroll
       for (int e = 0; e < 8; ++e) m8[e] = sv[e];
 #pragma unroll
-      for (int e = 8; e < 128; e += 16)
+      for (int e = 8; e < 120; e += 16)
 #pragma unroll
         for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m8[j] = fmaxf(m8[j], sv[120 + j]);
       const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
       const float m_cand = mx * scale_log2;
       const bool need = (t == 0) || (m_cand > m_ref + Cfg::RESCALE_THRESHOLD);
@@ -849,9 +851,11 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
       for (int e = 0; e < 8; ++e) m8[e] = sv[e];
 #pragma unroll
-      for (int e = 8; e < 128; e += 16)
+      for (int e = 8; e < 120; e += 16)
 #pragma unroll
         for (int jj = 0; jj < 8; ++jj) m8[jj] = fmax3(m8[jj], sv[e + jj], sv[e + 8 + jj]);
+#pragma unroll
+      for (int jj = 0; jj < 8; ++jj) m8[jj] = fmaxf(m8[jj], sv[120 + jj]);
       const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
       const float m_ref = mx * scale_log2;
       const uint64_t sc2 = f2_pack(scale_log2, scale_log2);

@@ -363,3 +363,16 @@ def test_the_result_may_be_written_over_the_queries(b, tq, tk, h, d, dtype):
         buf = q.contiguous().clone()
         assert ltx_nn.cross_attention(buf, k, v, h, mask=m, gate_logits=gate, out=buf) is buf
         assert torch.equal(buf, want)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("b,tq,tk,h,d", [(1, 300, 128, 2, 64), (1, 300, 128, 2, 128), (2, 200, 640, 2, 64),
+                                         (1, 700, 1000, 2, 128)])
+def test_rows_whose_scores_are_all_far_below_zero(b, tq, tk, h, d, masked):
+    """The row maximum is that of the row's own scores: anything else that entered it, a zero
+    say, would leave these rows (scores around -80) without any weight."""
+    g, q, k, v, _ = inputs(16, b, tq, tk, h, d, torch.bfloat16)
+    q, k = q.abs() + 0.5, (k * 0.5 - 80 / (1.3 * d * d ** -0.5)).contiguous()
+    m = torch.ones(b, tk, dtype=torch.bool, device=DEV)
+    got = ltx_nn.cross_attention(q, k, v, h, mask=m if masked else None)
+    check(got, q, k, v, h, ~m, None, None, d ** -0.5)
