@@ -298,15 +298,17 @@ class LTXModel(torch.nn.Module):
         inner = attn.heads * attn.dim_head
         wkv, bkv = attn.packed_kv()
         key = id(attn)
+        weights = [wkv.data_ptr(), *[_version(t) for t in (wkv, bkv, attn.to_k.weight, attn.to_k.bias, attn.to_v.weight,
+                                                           attn.to_v.bias, attn.k_norm.weight)]]
         hit = self._kv_cache.get(key)
         if hit is not None:
-            c_ref, c_ver, shape, w_ptr, kv = hit
-            if c_ref is src and c_ver == _version(src) and shape == tuple(ctx.shape) and w_ptr == wkv.data_ptr():
+            c_ref, c_ver, shape, made_with, kv = hit
+            if c_ref is src and c_ver == _version(src) and shape == tuple(ctx.shape) and made_with == weights:
                 return kv
         kv = torch.empty(ctx.shape[0], wkv.shape[0], device=ctx.device, dtype=ctx.dtype)
         nat.linear(ctx, wkv, kv, nat.epilogue(bias=bkv))
         attn._norm_rope(kv[:, :inner], rows, attn.k_norm.weight, None)
-        self._kv_cache[key] = (src, _version(src), tuple(ctx.shape), wkv.data_ptr(), kv)
+        self._kv_cache[key] = (src, _version(src), tuple(ctx.shape), weights, kv)
         return kv
 
     def cached_cat(self, a: torch.Tensor, b: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

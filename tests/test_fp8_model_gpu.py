@@ -348,3 +348,26 @@ def test_connector_block_runs_its_quantised_weights():
     assert sum(v["launches"] for k, v in calls.items() if "linear_fp8" in k) == 4
     assert not any(k.startswith("linear ") for k in calls)
     assert 1e-4 < rel_l2(got, want) < 0.15
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_a_cached_context_projection_follows_the_weights(quantised):
+    """The keys and values of a text context are kept over the denoise steps, not over a change
+    of the weights that made them."""
+    cfg = small_cfg()
+    model, _ = philox_model(cfg, 33, host_copy=False)
+    other, _ = philox_model(cfg, 34, host_copy=False)
+    if quantised:
+        model.quantize_fp8()
+        other.quantize_fp8()
+    video = video_inputs(cfg, torch.bfloat16)
+    model(video, None)
+    model.load_state_dict(other.state_dict())
+    assert torch.equal(model(video, None)[0], other(video, None)[0])
+    with torch.no_grad():
+        for m in (model, other):
+            for name, p in m.named_parameters():
+                if name.endswith(("attn2.to_k.bias", "attn2.to_v.weight", "attn2.k_norm.weight")):
+                    p.mul_(1.5)
+    other._kv_cache.clear()
+    assert torch.equal(model(video, None)[0], other(video, None)[0])
