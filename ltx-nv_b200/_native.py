@@ -704,6 +704,9 @@ def fp8_force_pair(pair: int) -> None:
     _call("ltx_test_fp8_force_pair", pair)
 
 
+_SIZES = {LTX_F32: 4, LTX_BF16: 2}  # bytes of an element
+
+
 def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilogue | None = None) -> None:
     """c = epilogue(quantize_fp8(x) @ w.T (+ bias)); x (M, K) float32 or bfloat16 with unit
     column stride, c (M, N) a row-major view in the epilogue's type, or any contiguous (..., N)
@@ -716,13 +719,13 @@ def quantize_linear_fp8(x: torch.Tensor, w: Fp8Rows, c: torch.Tensor, epi: Epilo
     if not c.numel():
         return
     lib = load_library()
+    px, pc = x.data_ptr(), c.data_ptr()
     n = lib.ltx_quantize_linear_fp8_workspace_bytes(m, k)
-    if n == 0:  # none is needed, unless the result may overwrite x
-        px, pc = x.data_ptr(), c.data_ptr()
-        if px < pc + ((m - 1) * ld + w.rows) * c.element_size() and pc < px + ((m - 1) * ldx + k) * x.element_size():
-            n = m * ((k + 15) // 16 * 16) + lib.ltx_fp8_scale_bytes(m, k)
+    # none is needed for a few rows, unless the result may overwrite x
+    if n == 0 and px < pc + ((m - 1) * ld + w.rows) * _SIZES[dt] and pc < px + ((m - 1) * ldx + k) * _SIZES[xdt]:
+        n = m * ((k + 15) // 16 * 16) + lib.ltx_fp8_scale_bytes(m, k)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _on(x, "ltx_quantize_linear_fp8", x.data_ptr(), ldx, xdt, *w.operand(), c.data_ptr(), ld, m, w.rows, k,
+    _on(x, "ltx_quantize_linear_fp8", px, ldx, xdt, *w.operand(), pc, ld, m, w.rows, k,
         ctypes.byref(epi) if epi is not None else None, ws.data_ptr() if n else None, n, dt,
         label=f"quantize_linear_fp8 M={m} N={w.rows} K={k}" if _profile is not None else None)
 
