@@ -520,7 +520,7 @@ def _version(t: torch.Tensor) -> int:
 
 
 def _requantize_fp8(module: "Fp8Module", _incompatible_keys) -> None:
-    for name in list(module.fp8):
+    for name in [n for n in module.fp8 if n in module._fp8_stamps]:
         module.weight8(name, module._fp8_weight(name), loaded=True)
 
 

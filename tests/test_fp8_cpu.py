@@ -350,7 +350,11 @@ def test_quantised_weights_follow_the_parameters(monkeypatch, inference):
     own = nat.Fp8Rows(64, 64, device="cpu")
     attn.fp8["own"] = own
     assert attn.weight8("own", attn.to_q.weight) is own
-    del attn.fp8["own"]
+    ff.fp8["own"] = own
+    for m in (attn, ff):
+        m.load_state_dict(m.state_dict())
+    assert attn.fp8["own"] is own and ff.fp8["own"] is own
+    del attn.fp8["own"], ff.fp8["own"]
     # not in the middle of a capture, which would quantise at every replay
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     merge(ff)
