@@ -651,7 +651,8 @@ class Fp8Rows:
         return out
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values in `dtype` (float32 or bfloat16; exact in both)."""
+        """The values in `dtype` (float32 or bfloat16; exact in both, but for values below
+        bfloat16's smallest, 2^-133, and above its largest)."""
         _same_device(self.buf)
         out = torch.empty(self.shape, dtype=dtype, device=self.buf.device)
         dt = _dt(out)

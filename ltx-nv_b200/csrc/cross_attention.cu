@@ -35,7 +35,9 @@ struct KeyMask {
   }
 };
 
-// One query per thread, key tiles of 32 in shared memory, online softmax in fp32.
+// One query per thread, key tiles of 32 in shared memory, online softmax in fp32. 2 x 16 heads
+// of 64, 256 keys, 1024 queries: 151 us, 14 TFLOP/s; the fp32 pipe is a third busy, since every
+// multiply-add takes its own shared-memory operand and every key rescales the D sums.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) masked_attn_simt_kernel(const T* __restrict__ Q, int64_t ldq,
                                                                const T* __restrict__ K, int64_t ldk,
@@ -376,6 +378,12 @@ void launch_masked_few(const void* q, int64_t ldq, const void* k, int64_t ldk, c
 // arithmetic, part of the exponentials on the FMA pipe, lazy rescaling: attention.cu).
 // TMEM as in attention.cu: head_dim 64 keeps P beside S (S_i is computed two tiles
 // ahead), head_dim 128 writes P over S.
+// P is rounded to bf16, the type that an MMA with bf16 V takes, as in attention.cu (the row sum
+// is not): 2^-8 of each weight at the most, 2.2e-3 rel-L2 of the result against float64, where
+// rounding the result alone gives 1.7e-3.
+// 2 x 6144 queries, 1024 keys, 32 heads of 64: 181 us with every key kept, 112 with half of them;
+// no unit is full (issue slots 44 %, special functions 39 %, tensor pipe 27 %): the two softmax
+// warps of a scheduler wait for tensor memory and barriers in turn.
 // split > 1 (few units, many key tiles): the CTAs of a cluster take shares of one unit's
 // list and merge their fp32 O / l and log-sum-exp through distributed shared memory, in
 // rank order.

@@ -359,6 +359,8 @@ template <> LTX_DEVICE void st4v<__nv_bfloat16>(__nv_bfloat16* p, const float (&
 template <> LTX_DEVICE void st4v<float>(float* p, const float (&v)[4]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
+// SiLU's division gives 0 where the divisor passes 2^126 (v below -87; the value is within
+// 2^-119 of 0 there).
 // Epilogue of W (1, 4 or 16) accumulators, columns [col, col + W) of row `row` (sample sb, token
 // st), in fp32 and rounded once on the store: acc + bias, then the activation, residual +
 // gate * (acc + bias), or + row_vec on marked rows. W > 1 needs every vector aligned there.

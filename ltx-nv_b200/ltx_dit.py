@@ -867,8 +867,9 @@ def av_cfg_denoise_step(model: LTXModel, v_latent: torch.Tensor, a_latent: torch
     the proj_out epilogues (ltx_dit.py:565-606 with CFG-only guidance).
 
     v_latent (1, Tv, C), a_latent (1, Ta, C), positions (1, 3, Tv, 2) / (1, 1, Ta, 2),
-    contexts (1, S, C_v) / (1, S_a, C_a). Returns (next video latent (1, Tv, C), next audio
-    latent (1, Ta, C))."""
+    contexts (1, S, C_v) / (1, S_a, C_a), every token of which takes part (padded ones:
+    guided_denoise_step, or Modality.context_mask). Returns (next video latent (1, Tv, C),
+    next audio latent (1, Ta, C))."""
     dtype = model.proj_out.weight.dtype
     dev = v_latent.device
     sigma, sigma_next = _sigma_pair(sigmas, idx)
@@ -907,7 +908,9 @@ class NativeStep:
     the path a C or C++ caller takes without Python. It owns an ltx_ctx (TMA descriptor
     cache, step workspace sized for T latent and S text tokens) and the weight table of
     `model` (the packed attention weights of ltx_nn). Video-only models without
-    cross-adaLN (3, 5). Results equal cfg_denoise_step bit for bit."""
+    cross-adaLN. It runs the parameters in their own type and
+    takes no context masks: results equal cfg_denoise_step bit for bit for a model without
+    quantize_fp8 and a call without masks."""
 
     def __init__(self, model: LTXModel, tokens: int, text_tokens: int):
         cfg = model.cfg
@@ -978,7 +981,8 @@ class NativeStep:
     def __call__(self, latent: torch.Tensor, positions: torch.Tensor, context_pos: torch.Tensor,
                  context_neg: torch.Tensor, sigmas: torch.Tensor, idx: int, cfg_scale: float,
                  keyframes_mask: torch.Tensor | None = None, reuse: bool = False, out: tuple | None = None):
-        """Same arguments and results as cfg_denoise_step. reuse=True keeps the RoPE tables
+        """cfg_denoise_step without context masks, on the unquantised parameters: the same
+        arguments and results otherwise. reuse=True keeps the RoPE tables
         and text K/V of the previous call (same positions and contexts). `out` optionally
         gives (velocity (2, T, C), denoised (1, T, C), next latent (1, T, C)) buffers."""
         sigma, sigma_next = _sigma_pair(sigmas, idx)

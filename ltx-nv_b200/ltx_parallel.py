@@ -253,7 +253,8 @@ class SequenceParallel:
 
 
 class ParallelDenoiser:
-    """CFG x SP execution of ltx_dit.cfg_denoise_step across the default process group."""
+    """CFG x SP execution of ltx_dit.cfg_denoise_step across the default process group,
+    without context masks."""
 
     def __init__(self, model: ltx_dit.LTXModel, cfg_split: int | None = None, exchange: str = "auto"):
         """exchange: "peer" runs the Ulysses exchange inside the q/k and attention kernels
