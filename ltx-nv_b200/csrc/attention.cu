@@ -367,22 +367,24 @@ __device__ __forceinline__ void fmha_body(const CUtensorMap* tmQ_, const CUtenso
         for (int e = 0; e < 128; ++e)
           if (e >= valid) sv[e] = -INFINITY;
       }
-      // row max: 3-input max, 8 independent chains
+      // row max: 3-input max, 8 independent chains; it keeps a NaN, which the cubic below would lose,
+      // and m_ref carries it into every weight of the row
       float m8[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) m8[e] = sv[e];
 #pragma unroll
       for (int e = 8; e < 120; e += 16)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], sv[e + j], sv[e + 8 + j]);
+        for (int j = 0; j < 8; ++j) m8[j] = fmax3_nan(m8[j], sv[e + j], sv[e + 8 + j]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m8[j] = fmaxf(m8[j], sv[120 + j]);
-      const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+      for (int j = 0; j < 8; ++j) m8[j] = fmax3_nan(m8[j], sv[120 + j], sv[120 + j]);
+      const float mx =
+          fmax3_nan(fmax3_nan(m8[0], m8[1], m8[2]), fmax3_nan(m8[3], m8[4], m8[5]), fmax3_nan(m8[6], m8[7], m8[7]));
       const float m_cand = mx * scale_log2;
-      const bool need = (t == 0) || (m_cand > m_ref + Cfg::RESCALE_THRESHOLD);
+      const bool need = (t == 0) || !(m_cand <= m_ref + Cfg::RESCALE_THRESHOLD);
       float alpha = 1.f;
       if (need) {
-        const float m_new = fmaxf(m_ref, m_cand);
+        const float m_new = fmax3_nan(m_ref, m_cand, m_cand);
         alpha = (t == 0) ? 0.f : ex2_approx(m_ref - m_new);
         m_ref = m_new;
       }

@@ -376,3 +376,26 @@ def test_rows_whose_scores_are_all_far_below_zero(b, tq, tk, h, d, masked):
     m = torch.ones(b, tk, dtype=torch.bool, device=DEV)
     got = ltx_nn.cross_attention(q, k, v, h, mask=m if masked else None)
     check(got, q, k, v, h, ~m, None, None, d ** -0.5)
+
+
+@pytest.mark.parametrize("parts", [0, 3])
+@pytest.mark.parametrize("tq,tk", [(40, 128), (300, 256), (300, 500)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_at_every_key_reaches_its_head_without_a_mask(d, tq, tk, parts):
+    """The same without a mask, in whole units and in parts of a unit's keys."""
+    b, h = 1, 2
+    g, q, k, v, _ = inputs(14, b, tq, tk, h, d, torch.bfloat16)
+    nat.attention_force_split(parts)
+    try:
+        clean = ltx_nn.cross_attention(q, k, v, h)
+        lost = []
+        for key in (*range(128), *range(128, tk, 37)):
+            k2 = k.clone()
+            k2[0, key, key % d] = math.nan
+            got = ltx_nn.cross_attention(q, k2, v, h)
+            if not (torch.isnan(got[..., :d]).all() and torch.equal(got[..., d:], clean[..., d:])):
+                lost.append(key)
+        assert not lost, lost
+    finally:
+        nat.attention_force_split(0)
+    assert nat.device_error_flags() == 0
