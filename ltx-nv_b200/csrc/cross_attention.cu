@@ -438,10 +438,11 @@ struct MaUnit {
   uint32_t marked[2];
   uint32_t pad2[2];
 };
-// A row with a finite score has a sum of weights of at least 2^-8 (m_ref is at most the
-// taken from weighs 1, and m_ref only rises with the next such key); one of -inf scores alone
-// has the remainders of the cubic, 36 * 19 * 2^-149 a tile. Below kMaDeadRow there is no weight.
-constexpr float kMaDeadRow = 0x1p-100f;
+// The sum of weights below which a row has none. The key that m_ref was taken from weighs 1 (at
+// scores of 1e9, where a product's rounding shows, 2^-60), and m_ref only rises with the next
+// such key; a row of -inf scores alone sums the cubic's remainders, 36 * 19 * 2^-149 a tile, over
+// at most 4096 tiles.
+constexpr float kMaDeadRow = 0x1p-126f;
 constexpr int kMaUnits = 4;  // units the producer may be ahead
 
 LTX_DEVICE void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

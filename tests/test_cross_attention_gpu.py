@@ -399,3 +399,21 @@ def test_nan_at_every_key_reaches_its_head_without_a_mask(d, tq, tk, parts):
     finally:
         nat.attention_force_split(0)
     assert nat.device_error_flags() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_equal_scores_average_the_values(d):
+    """Keys that are all alike weigh the same, whatever their score: up to 1.2e9 in log2 units
+    the rounding of the maximum is below 2^-24 of it, a factor of 2^72 that cancels."""
+    b, tq, tk, h = 1, 300, 256, 2
+    g, q, k, v, _ = inputs(18, b, tq, tk, h, d, torch.bfloat16)
+    k = k[:, :1].expand(b, tk, h * d)
+    m = torch.ones(b, tk, dtype=torch.bool, device=DEV)
+    mean = v.double().mean(1, keepdim=True)
+    size = v.double().abs().mean(1, keepdim=True)
+    for scale in (1.0, 3e2, 3e4, 1e6, 3e6):
+        top = (q.double().abs() @ k[0, 0].double().abs()).max().item() * 200.0 * scale * d ** -0.5 * 1.4427
+        if top > 1.2e9:
+            continue
+        got = ltx_nn.cross_attention((q * 200.0).contiguous(), k, v, h, mask=m, scale=scale * d ** -0.5).double()
+        assert ((got - mean).abs() <= size * (2.0 ** -8 + 2.0 ** -12) + mean.abs() * 2.0 ** -8).all(), scale
